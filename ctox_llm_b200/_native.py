@@ -158,6 +158,64 @@ class FusedMatVecOp(C.Structure):
     ]
 
 
+MAX_BATCH = 2048
+PAGES_NONE_FREE, PAGES_ROW_FULL, PAGES_TOO_MANY, PAGES_BAD_INPUT = 1, 2, 4, 8
+ROPE_HALF, ROPE_ADJACENT = 0, 1
+
+
+def _fields(kind, names):
+    return [(n, kind) for n in names.split()]
+
+
+class PagedKV(C.Structure):
+    """ctox_paged_kv (include/ctox_b200.h): a K/V cache in pages. Pointers are device addresses."""
+
+    _fields_ = (_fields(C.c_void_p, "k v") + _fields(C.c_uint32, "dtype page_tokens n_pages") +
+                _fields(C.c_uint64, "page_stride token_stride head_stride"))
+
+
+class PageSlots(C.Structure):
+    """ctox_page_slots_op (include/ctox_b200.h)."""
+
+    _fields_ = (_fields(C.c_uint32, "n_requests page_tokens n_pages table_rows max_pages n_tokens") +
+                _fields(C.c_void_p, "new_tokens rows kv_lens_in kv_lens_out block_table") +
+                _fields(C.c_uint64, "table_stride") +
+                _fields(C.c_void_p, "free_pages free_count_in free_count_out query_offsets slots positions requests status"))
+
+
+class PageRelease(C.Structure):
+    """ctox_page_release_op (include/ctox_b200.h)."""
+
+    _fields_ = (_fields(C.c_uint32, "n_requests page_tokens n_pages table_rows max_pages") +
+                _fields(C.c_void_p, "rows kv_lens block_table") + _fields(C.c_uint64, "table_stride") +
+                _fields(C.c_void_p, "free_pages free_count_in free_count_out status"))
+
+
+class RopeAppend(C.Structure):
+    """ctox_rope_append_op (include/ctox_b200.h). `axis`: the axis of each pair, as bytes or numbers."""
+
+    _fields_ = (_fields(C.c_uint32, "tokens heads kv_heads dim rot_dim axes pairing source_dtype") +
+                [("rope_base", C.c_double), ("axis", C.c_uint8 * 128), ("positions", C.c_void_p), ("position_stride", C.c_uint64)] +
+                _fields(C.c_void_p, "q k v") +
+                _fields(C.c_uint64, "q_token_stride q_head_stride k_token_stride k_head_stride v_token_stride v_head_stride") +
+                _fields(C.c_void_p, "q_norm k_norm") + _fields(C.c_float, "norm_offset norm_eps") + [("q_out", C.c_void_p)] +
+                _fields(C.c_uint64, "q_out_token_stride q_out_head_stride") + [("slots", C.c_void_p), ("kv", PagedKV)])
+
+    def __init__(self, axis=(), **fields):
+        super().__init__(axis=(C.c_uint8 * 128)(*axis), **fields)
+
+
+class PagedAttention(C.Structure):
+    """ctox_paged_attention_op (include/ctox_b200.h)."""
+
+    _fields_ = (_fields(C.c_uint32, "n_requests n_tokens max_new_tokens max_kv_tokens heads kv_heads dim causal window") +
+                [("scale", C.c_float)] + _fields(C.c_void_p, "query_offsets kv_lens rows block_table") +
+                _fields(C.c_uint32, "table_rows max_pages") + _fields(C.c_uint64, "table_stride") + _fields(C.c_void_p, "sinks q") +
+                _fields(C.c_uint64, "q_token_stride q_head_stride") + [("out", C.c_void_p)] +
+                _fields(C.c_uint64, "out_token_stride out_head_stride") + [("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+                                                                          ("kv", PagedKV)])
+
+
 # name -> (restype, argtypes); every symbol of include/ctox_b200.h
 SIGNATURES = {
     "ctox_abi_version": (C.c_uint32, []),
@@ -203,6 +261,11 @@ SIGNATURES = {
     "ctox_gated_delta_scan_layers": (C.c_int32, [C.c_void_p] + [C.c_void_p] * 8 + [C.c_uint32] * 4),
     "ctox_gated_delta_scan_f16_state": (C.c_int32, [C.c_void_p] + [C.c_void_p] * 8 + [C.c_uint32] * 5),
     "ctox_gated_delta_prepare": (C.c_int32, [C.c_void_p] + [C.c_void_p] * 6 + [C.c_uint32] * 2),
+    "ctox_page_slots": (C.c_int32, [C.c_void_p, C.POINTER(PageSlots)]),
+    "ctox_page_release": (C.c_int32, [C.c_void_p, C.POINTER(PageRelease)]),
+    "ctox_rope_append": (C.c_int32, [C.c_void_p, C.POINTER(RopeAppend)]),
+    "ctox_paged_attention_workspace": (C.c_int32, [C.c_void_p, C.POINTER(PagedAttention), C.POINTER(C.c_uint64)]),
+    "ctox_paged_attention": (C.c_int32, [C.c_void_p, C.POINTER(PagedAttention)]),
     "ctox_argmax_f32": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p]),
     "ctox_argmax_f32_host": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p,
                                          C.POINTER(C.c_uint32)]),

@@ -207,6 +207,29 @@ class B200Backend:
             self._ctx, *(C.c_void_p(x) for x in (a, b, a_log, dt_bias, log_decay, beta)), tokens,
             heads))
 
+    # -- a paged K/V cache that many requests share (include/ctox_b200.h; device addresses) ----
+    def page_slots(self, operation: N.PageSlots) -> None:
+        """Pages, slots and positions of every request's new tokens."""
+        self._check(self._lib.ctox_page_slots(self._ctx, operation))
+
+    def page_release(self, operation: N.PageRelease) -> None:
+        """The pages of finished requests go back onto the stack of free ones."""
+        self._check(self._lib.ctox_page_release(self._ctx, operation))
+
+    def rope_append(self, operation: N.RopeAppend) -> None:
+        """Norm and rotation of a layer's queries and keys; keys and values into the cache."""
+        self._check(self._lib.ctox_rope_append(self._ctx, operation))
+
+    def paged_attention_workspace(self, operation: N.PagedAttention) -> int:
+        """Bytes of workspace for any call with the operation's heads, kv_heads and dim."""
+        v = C.c_uint64()
+        self._check(self._lib.ctox_paged_attention_workspace(self._ctx, operation, C.byref(v)))
+        return v.value
+
+    def paged_attention(self, operation: N.PagedAttention) -> None:
+        """Every request's new tokens attend to what it has in the cache."""
+        self._check(self._lib.ctox_paged_attention(self._ctx, operation))
+
     # -- selection ------------------------------------------------------------------------
     def argmax(self, logits_ptr: int, n: int, row_ids_ptr: int = 0) -> int:
         """Greedy token over device logits: last maximal index under f32::total_cmp

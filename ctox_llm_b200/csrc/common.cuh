@@ -185,6 +185,7 @@ enum : int32_t {
     DEV_ERR_WAIT_TIMEOUT = 1,   // a bounded mbarrier wait ran out
     DEV_ERR_NONFINITE_SCALE = 2,
     DEV_ERR_NONFINITE_VALUE = 3,
+    DEV_ERR_BAD_INDEX = 4,  // a page, slot, row or length outside its bounds
 };
 
 inline float f16_bits_to_f32(uint16_t h) {

@@ -1,0 +1,104 @@
+// Shared parts of the operators over a paged K/V cache that many requests use: argument checks, device access.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "paged_plan.cuh"
+
+namespace ctox {
+namespace paged {
+
+inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+inline ctox_status check_kv(ctox_ctx *ctx, const ctox_paged_kv &kv, uint32_t kv_heads, const char *what) {
+    if (!kv.k || !kv.v || !aligned16(kv.k) || !aligned16(kv.v))
+        return fail(ctx, CTOX_SHAPE, "%s: k and v of the cache are device addresses aligned to 16 bytes", what);
+    if (kv.dtype != CTOX_BF16 && kv.dtype != CTOX_F16) return fail(ctx, CTOX_UNSUPPORTED_DTYPE, "%s: cache of dtype %u", what, kv.dtype);
+    if (!kv.page_tokens || kv.page_tokens % 16 || !kv.n_pages || (uint64_t)kv.n_pages * kv.page_tokens > 0x7fffffffull)
+        return fail(ctx, CTOX_SHAPE, "%s: %u pages of %u tokens (a multiple of 16, below 2^31 tokens in all)", what, kv.n_pages,
+                    kv.page_tokens);
+    if (kv.page_stride % 8 || kv.token_stride % 8 || kv.head_stride % 8 || !kv.page_stride || !kv.token_stride ||
+        (kv_heads > 1 && !kv.head_stride))
+        return fail(ctx, CTOX_SHAPE, "%s: cache strides %llu, %llu, %llu are not multiples of 8 elements", what,
+                    (unsigned long long)kv.page_stride, (unsigned long long)kv.token_stride, (unsigned long long)kv.head_stride);
+    if (kv_heads > 1 && kv.page_stride % kv.head_stride)
+        return fail(ctx, CTOX_SHAPE, "%s: page stride %llu is not a multiple of the head stride %llu", what,
+                    (unsigned long long)kv.page_stride, (unsigned long long)kv.head_stride);
+    return CTOX_OK;
+}
+inline ctox_status check_dim(ctox_ctx *ctx, uint32_t dim, const char *what) {
+    if (dim != 64 && dim != 128 && dim != 256) return fail(ctx, CTOX_SHAPE, "%s: heads of %u dimensions (64, 128 or 256)", what, dim);
+    return CTOX_OK;
+}
+
+// Work goes to the context's device, whichever is current in the calling thread; that one is current again afterwards.
+class DeviceGuard {
+    int before_ = -1;
+    cudaError_t error_ = cudaSuccess;
+
+  public:
+    explicit DeviceGuard(int device) {
+        error_ = cudaGetDevice(&before_);
+        if (error_ == cudaSuccess && before_ != device)
+            error_ = cudaSetDevice(device);
+        else
+            before_ = -1;
+    }
+    ~DeviceGuard() {
+        if (before_ >= 0) cudaSetDevice(before_);
+    }
+    cudaError_t error() const { return error_; }
+};
+
+#ifdef __CUDACC__
+// Index out of range on the device: the caller leaves the access out.
+__device__ __forceinline__ void bad_index(int32_t *error_word) { *reinterpret_cast<volatile int32_t *>(error_word) = DEV_ERR_BAD_INDEX; }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Inclusive sum over the block's threads in order; `warps` holds one word per warp.
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, V *warps) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= (uint32_t)o) v += u;
+    }
+    __syncthreads();  // `warps` may still be read from the sum before
+    if (lane == 31) warps[warp] = v;
+    __syncthreads();
+    V before = 0;
+    for (uint32_t w = 0; w < warp; ++w) before += warps[w];
+    return v + before;
+}
+// Last i in [0, n) with at[i] <= x; at[0] <= x.
+template <typename V>
+__device__ __forceinline__ uint32_t last_at_most(const V *at, uint32_t n, V x) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (at[mid] <= x)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+#endif
+
+}  // namespace paged
+}  // namespace ctox

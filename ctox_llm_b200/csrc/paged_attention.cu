@@ -1,0 +1,550 @@
+// Attention over a paged K/V cache for requests with few rows (a decode step, a verify pass of a few drafts), the merge of what
+// CTAs share, and the entry points.
+//
+// With up to sixteen rows per KV head the work is the cache's bytes: about 1 flop per byte and row, so the kernel is built
+// around the stream. A persistent CTA per SM takes an equal share of all requests' key tiles (paged_plan.cuh). One warp copies
+// tiles of K and V into a ring of three by TMA (whole pages' boxes, three quarters of shared memory in flight); the others
+// compute while the next tiles are on their way: scores as K Q^T, sixteen keys by eight rows per mma, so that the rows, not the keys, are
+// padded to eight; one barrier per tile to exchange the scores; then every warp forms the weights that its share of the head's dimensions needs
+// (lane = row, redundantly: 32 exponentials per lane and tile) and adds V^T P for those dimensions. No output or maximum ever
+// crosses a warp.
+#include "paged_attention.cuh"
+
+#include <cmath>
+
+namespace ctox {
+namespace paged {
+namespace {
+
+constexpr int kStages = 3;
+constexpr uint32_t kMostCtas = 160;  // one per SM
+
+template <int D, int NT>
+struct Rows {
+    static constexpr int KT = D == 256 ? 64 : 128;         // keys of a tile
+    static constexpr int NW = D == 64 ? 4 : 8;             // computing warps
+    static constexpr int BR = NT * 8;                      // rows of a unit
+    static constexpr int KM = KT / 16;                     // score tiles of sixteen keys
+    static constexpr int SPLIT = NW > KM ? NW / KM : 1;    // of a head's dimensions among warps, for the scores
+    static constexpr int MW = KM * SPLIT / NW;             // score tiles per warp
+    static constexpr int KSTEPS = D / 16 / SPLIT;          // products of a score tile
+    static constexpr int DW = D * NT / NW;                 // dimensions of a warp's output, for one group of eight rows
+    static constexpr int SP = KT + 8;                      // row pitch of the scores: keys and rows fall into different banks
+    static constexpr uint32_t TILE = KT * D * 2;           // bytes of K or V
+    static constexpr size_t SCORES = 2ull * SPLIT * BR * SP * 4;
+    static size_t smem(uint32_t n) { return 1024 + (size_t)kStages * 2 * TILE + SCORES + (n + 1) * 8; }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(Rows<D, NT>::NW * 32 + 32)
+    k_attention_rows(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a,
+                     int32_t *error_word) {
+    using namespace umma;
+    using R = Rows<D, NT>;
+    constexpr uint32_t NCH = D / 64;
+    extern __shared__ uint8_t raw[];
+    __shared__ __align__(8) uint64_t bars[2 * kStages];
+    __shared__ unsigned long long scan[32];
+    __shared__ volatile int dead;
+    __shared__ Cut cuts[2];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+    uint8_t *aligned = raw + (base - smem_addr(raw));
+    float *scores = reinterpret_cast<float *>(aligned + kStages * 2 * R::TILE);
+    unsigned long long *at = reinterpret_cast<unsigned long long *>(aligned + kStages * 2 * R::TILE + R::SCORES);
+    const uint32_t full = smem_addr(bars), empty = full + kStages * 8;
+    if (tid == 0) {
+        dead = 0;
+        for (uint32_t i = 0; i < kStages; ++i) {
+            bar_init(full + i * 8, 1);
+            bar_init(empty + i * 8, R::NW);
+        }
+        bar_init_fence();
+    }
+    __syncthreads();
+    pdl_launch();
+    pdl_wait();
+    const uint64_t total = lay_line(a, at, scan, error_word);
+    const uint32_t pieces = total ? pieces_of(total, gridDim.x, a.least) : 0;
+    const Line line{a, at, a.op.n_requests};
+    if (blockIdx.x >= pieces) {
+        if (tid == 0) a.shared[blockIdx.x].sharers = 0;
+        return;
+    }
+    if (warp < 2) {
+        const Cut c = cut_at(a.shape, line, total, pieces, blockIdx.x + warp, a.least);
+        if (lane == 0) cuts[warp] = c;
+    }
+    __syncthreads();
+    Walk w;
+    w.at = cuts[0];
+    w.end = cuts[1].x;
+    bool ok = true;
+    if (warp == R::NW) {  // the copies: a lane per box
+        const uint32_t per = R::KT / a.box, box_bytes = a.box * D * 2;
+        uint32_t n = 0;
+        for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
+            const int32_t *table = table_row(a, w.at.request);
+            for (uint32_t t = w.tile0; t < w.tile1; ++t, ++n) {
+                const uint32_t s = n % kStages, round = n / kStages;
+                const uint32_t token = (w.u.tile0 + t) * R::KT + lane * a.box;
+                int32_t page = -1;
+                bool mine = lane < per && token < w.u.hi && token + a.box > w.u.lo;
+                if (mine) mine = page_at(a, table, token, page, error_word);
+                const uint32_t copies = __popc(__ballot_sync(0xffffffffu, mine));
+                if (round > 0 && !(ok = __all_sync(0xffffffffu, bar_wait(empty + s * 8, (round - 1) & 1, &dead)))) break;
+                if (lane == 0) bar_expect(full + s * 8, copies * 2 * box_bytes);
+                __syncwarp();
+                if (mine) {
+                    const int group = (int)(token % a.op.kv.page_tokens / 8), step = box_step(a, page, w.at.head);
+                    const uint32_t dst = base + s * 2 * R::TILE + lane * box_bytes;
+                    load_box(dst, &map_k, full + s * 8, 0, group, step);
+                    load_box(dst + R::TILE, &map_v, full + s * 8, 0, group, step);
+                }
+            }
+        }
+        if (!ok && lane == 0) {  // leave no copy in flight behind
+            *error_word = DEV_ERR_WAIT_TIMEOUT;
+            for (uint32_t s = 0; s < kStages && s < n; ++s) bar_drain(full + s * 8, ((n - 1 - s) / kStages) & 1);
+        }
+        return;
+    }
+    // scores: this warp's tiles of sixteen keys and part of the dimensions; output: its group of rows and dimensions
+    const uint32_t part = R::SPLIT > 1 ? warp / R::KM : 0, key_tile0 = R::SPLIT > 1 ? warp % R::KM : warp;
+    constexpr uint32_t per_group = R::NW / NT;
+    const uint32_t group8 = warp / per_group, d_base = warp % per_group * R::DW;
+    const uint32_t quad = lane >> 2, c2 = (lane & 3) * 2;
+    // ldmatrix addresses inside a tile: key (row) and 16-byte column of this lane
+    const uint32_t k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_col = lane >> 4;
+    const uint32_t v_row = (lane & 7) + (lane >> 4) * 8, v_col = (lane >> 3) & 1;
+    bool shares = false;
+    uint32_t n = 0;
+    // Once a wait has run out of time (ok false) the warps go on without waiting, over whatever shared memory holds: all of
+    // them take the same trips, so the barriers below still meet.
+    for (; walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
+        const uint32_t group = a.shape.group;
+        // queries as the products' second operand, rows of the unit's block
+        uint32_t qf[NT][R::KSTEPS][2];
+#pragma unroll
+        for (int g = 0; g < NT; ++g) {
+            const uint32_t r = w.u.row0 + g * 8 + quad;
+            const T *q = nullptr;
+            if (g * 8 + quad < w.u.rows)
+                q = (const T *)a.op.q + (uint64_t)(w.q.q0 + r / group) * a.op.q_token_stride +
+                    (uint64_t)(w.at.head * group + r % group) * a.op.q_head_stride + part * (R::KSTEPS * 16) + c2;
+#pragma unroll
+            for (int k = 0; k < R::KSTEPS; ++k) {
+                qf[g][k][0] = q ? *reinterpret_cast<const uint32_t *>(q + k * 16) : 0;
+                qf[g][k][1] = q ? *reinterpret_cast<const uint32_t *>(q + k * 16 + 8) : 0;
+            }
+        }
+        // what this lane's row of the softmax sees
+        uint32_t row_lo = 0, row_hi = 0, all_lo = 0, all_hi = w.q.kv;  // all_*: what every row sees
+        {
+            const uint32_t in = group8 * 8 + quad;
+            if (in < w.u.rows) key_range(a.shape, w.q, w.u.row0 + in, w.u.row0 + in + 1, row_lo, row_hi);
+            uint32_t x;
+            key_range(a.shape, w.q, w.u.row0, w.u.row0 + 1, x, all_hi);
+            key_range(a.shape, w.q, w.u.row0 + w.u.rows - 1, w.u.row0 + w.u.rows, all_lo, x);
+        }
+        float top = -INFINITY, sum = 0.f;
+        float o[R::DW / 16][4];
+#pragma unroll
+        for (int i = 0; i < R::DW / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+        for (uint32_t t = w.tile0; t < w.tile1; ++t, ++n) {
+            const uint32_t s = n % kStages, key0 = (w.u.tile0 + t) * R::KT;
+            ok = ok && __all_sync(0xffffffffu, bar_wait(full + s * 8, (n / kStages) & 1, &dead));
+            const uint32_t kt = base + s * 2 * R::TILE, vt = kt + R::TILE;
+            float *buf = scores + (n & 1) * (R::SPLIT * R::BR * R::SP);
+#pragma unroll
+            for (int m = 0; m < R::MW; ++m) {
+                const uint32_t mt = key_tile0 + m * R::NW;
+                float acc[NT][2][4];
+#pragma unroll
+                for (int g = 0; g < NT; ++g)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[g][0][j] = acc[g][1][j] = 0.f;
+                const uint32_t key = mt * 16 + k_row, row = kt + (key >> 3) * (NCH * 1024) + (key & 7) * 128;
+#pragma unroll
+                for (int k = 0; k < R::KSTEPS; ++k) {
+                    const uint32_t col = part * (R::KSTEPS * 2) + k * 2 + k_col;  // of 16 bytes
+                    uint32_t f[4];
+                    ldmatrix4(f, row + (col >> 3) * 1024 + (((col & 7) ^ (key & 7)) << 4));
+#pragma unroll
+                    for (int g = 0; g < NT; ++g) mma16816<T>(acc[g][k & 1], f, qf[g][k][0], qf[g][k][1]);
+                }
+#pragma unroll
+                for (int g = 0; g < NT; ++g) {
+                    float *p = buf + (part * R::BR + g * 8 + c2) * R::SP + mt * 16 + quad;
+                    p[0] = acc[g][0][0] + acc[g][1][0];
+                    p[R::SP] = acc[g][0][1] + acc[g][1][1];
+                    p[8] = acc[g][0][2] + acc[g][1][2];
+                    p[R::SP + 8] = acc[g][0][3] + acc[g][1][3];
+                }
+            }
+            // one barrier per tile: the scores have two buffers, and a warp that writes the one two tiles on has seen all
+            // others arrive here for the tile between
+            asm volatile("bar.sync 1, %0;" ::"r"(R::NW * 32) : "memory");
+            float p[R::KM][4];
+            float mx = -INFINITY;
+            const bool whole = key0 >= all_lo && key0 + R::KT <= all_hi;
+            const float *row = buf + (group8 * 8 + quad) * R::SP + c2;
+#pragma unroll
+            for (int k = 0; k < R::KM; ++k) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float2 x = *reinterpret_cast<const float2 *>(row + k * 16 + h * 8);
+                    if (R::SPLIT > 1) {
+                        const float2 y = *reinterpret_cast<const float2 *>(row + R::BR * R::SP + k * 16 + h * 8);
+                        x.x += y.x;
+                        x.y += y.y;
+                    }
+                    p[k][2 * h] = x.x;
+                    p[k][2 * h + 1] = x.y;
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int k = 0; k < R::KM; ++k)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t key = key0 + k * 16 + (j >> 1) * 8 + c2 + (j & 1);
+                        if (key < row_lo || key >= row_hi) p[k][j] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int k = 0; k < R::KM; ++k) mx = fmaxf(fmaxf(mx, fmaxf(p[k][0], p[k][1])), fmaxf(p[k][2], p[k][3]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            mx *= a.c;
+            if (__any_sync(0xffffffffu, mx > top)) {
+                const float now = fmaxf(top, mx);
+                const float f = now == -INFINITY ? 1.f : ex2(top - now);  // nothing seen yet: 0
+                top = now;
+                sum *= f;
+                const float f0 = __shfl_sync(0xffffffffu, f, c2 * 4), f1 = __shfl_sync(0xffffffffu, f, c2 * 4 + 4);
+#pragma unroll
+                for (int i = 0; i < R::DW / 16; ++i) {
+                    o[i][0] *= f0;
+                    o[i][1] *= f1;
+                    o[i][2] *= f0;
+                    o[i][3] *= f1;
+                }
+            }
+            const float ref = top == -INFINITY ? 0.f : top;
+            float part_sum[2] = {0.f, 0.f};
+            uint32_t b[R::KM][2];
+#pragma unroll
+            for (int k = 0; k < R::KM; ++k) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    p[k][j] = ex2(fmaf(p[k][j], a.c, -ref));
+                    part_sum[j & 1] += p[k][j];
+                }
+                b[k][0] = pack_pair<T>(p[k][0], p[k][1]);
+                b[k][1] = pack_pair<T>(p[k][2], p[k][3]);
+            }
+            sum += part_sum[0] + part_sum[1];
+#pragma unroll
+            for (int k = 0; k < R::KM; ++k) {
+                const uint32_t key = k * 16 + v_row, vrow = vt + (key >> 3) * (NCH * 1024) + (key & 7) * 128;
+                uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+                if (!whole) {  // what lies in places that no row sees may be anything, and 0 times that is not 0
+                    const uint32_t x = key0 + k * 16 + c2;
+                    auto seen = [&](uint32_t t) { return t >= w.u.lo && t < w.u.hi; };
+                    keep0 = (seen(x) ? 0xffffu : 0) | (seen(x + 1) ? 0xffff0000u : 0);
+                    keep1 = (seen(x + 8) ? 0xffffu : 0) | (seen(x + 9) ? 0xffff0000u : 0);
+                }
+#pragma unroll
+                for (int i = 0; i < R::DW / 16; ++i) {
+                    const uint32_t col = (d_base + i * 16) / 8 + v_col;
+                    uint32_t f[4];
+                    ldmatrix4_t(f, vrow + (col >> 3) * 1024 + (((col & 7) ^ (key & 7)) << 4));
+                    if (!whole) {
+                        f[0] &= keep0;
+                        f[1] &= keep0;
+                        f[2] &= keep1;
+                        f[3] &= keep1;
+                    }
+                    mma16816<T>(o[i], f, b[k][0], b[k][1]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) bar_arrive(empty + s * 8);
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (w.begins && w.ends) {
+            const uint32_t in = group8 * 8 + quad, r = w.u.row0 + in;
+            const uint32_t head = w.at.head * group + r % group;
+            float inv = 0.f;
+            if (in < w.u.rows && sum != 0.f) {
+                if (a.op.sinks) sum += ex2(fmaf(a.op.sinks[head], 1.4426950408889634f, -top));
+                inv = 1.0f / sum;
+            }
+            const float i0 = __shfl_sync(0xffffffffu, inv, c2 * 4), i1 = __shfl_sync(0xffffffffu, inv, c2 * 4 + 4);
+            T *out = (T *)a.op.out + (uint64_t)(w.q.q0 + r / group) * a.op.out_token_stride + (uint64_t)head * a.op.out_head_stride + d_base + c2;
+#pragma unroll
+            for (int i = 0; i < R::DW / 16; ++i) {
+                const uint32_t x = transpose8(pack_pair<T>(o[i][0] * i0, o[i][1] * i1)), y = transpose8(pack_pair<T>(o[i][2] * i0, o[i][3] * i1));
+                if (in < w.u.rows) {
+                    *reinterpret_cast<uint32_t *>(out + i * 16) = x;
+                    *reinterpret_cast<uint32_t *>(out + i * 16 + 8) = y;
+                }
+            }
+        } else {
+            float *slot = a.partial + (blockIdx.x * 2ull + (w.begins ? 1 : 0)) * slot_floats(R::BR, D);
+            if (d_base == 0 && (lane & 3) == 0) {
+                slot[group8 * 8 + quad] = top;
+                slot[R::BR + group8 * 8 + quad] = sum;
+            }
+            slot += 2 * R::BR;
+#pragma unroll
+            for (int i = 0; i < R::DW / 16; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t d = d_base + i * 16 + quad + (j >> 1) * 8, r = group8 * 8 + c2 + (j & 1);
+                    slot[((d >> 2) * R::BR + r) * 4 + (d & 3)] = o[i][j];
+                }
+            if (w.begins) {
+                shares = true;
+                if (tid == 0)
+                    a.shared[blockIdx.x] = Shared{sharers(total, pieces, blockIdx.x, w.at.start + w.u.cost), w.at.request, w.at.head, w.u.row0, w.u.rows};
+            }
+        }
+    }
+    if (!shares && tid == 0) a.shared[blockIdx.x].sharers = 0;
+    if (!ok && lane == 0) *error_word = DEV_ERR_WAIT_TIMEOUT;
+}
+
+// What several CTAs share. Each holds the maximum, sum and output of its keys; with M the largest maximum, weights 2^(m - M) bring
+// them to one scale, in the order of the CTAs. A block takes 1024 / D rows of one unit, four dimensions per thread; its weights once
+// in shared memory.
+constexpr uint32_t kMergeThreads = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kMergeThreads) k_attention_merge(const __grid_constant__ AttnArgs a) {
+    __shared__ float weight[kMostCtas][16];
+    __shared__ float scale[16];
+    const uint32_t D = a.op.dim, BR = a.shape.block_rows, per = 4 * kMergeThreads / D, row_first = blockIdx.y * per;
+    pdl_launch();
+    pdl_wait();
+    const Shared s = a.shared[blockIdx.x];
+    if (!s.sharers || row_first >= s.rows) return;
+    const uint64_t slot = slot_floats(BR, D);
+    auto slot_of = [&](uint32_t i) { return a.partial + ((uint64_t)(blockIdx.x + i) * 2 + (i ? 0 : 1)) * slot; };
+    Request q;
+    read_request(a, s.request, q);
+    const uint32_t tid = threadIdx.x, group = a.shape.group;
+    for (uint32_t i = tid; i < s.sharers * per; i += kMergeThreads)
+        if (row_first + i % per < s.rows) weight[i / per][i % per] = slot_of(i / per)[row_first + i % per];
+    __syncthreads();
+    if (tid < per && row_first + tid < s.rows) {
+        float top = -INFINITY;
+        for (uint32_t i = 0; i < s.sharers; ++i) top = fmaxf(top, weight[i][tid]);
+        float sum = 0.f;
+        for (uint32_t i = 0; i < s.sharers; ++i) {
+            const float l = slot_of(i)[BR + row_first + tid];
+            // a part that saw nothing for this row has sum 0
+            const float f = l == 0.f ? 0.f : umma::ex2(weight[i][tid] - top);
+            weight[i][tid] = f;
+            if (l != 0.f) sum += f * l;
+        }
+        const uint32_t r = s.row0 + row_first + tid;
+        if (sum != 0.f && a.op.sinks)
+            sum += umma::ex2(fmaf(a.op.sinks[s.head * group + r % group], 1.4426950408889634f, -top));
+        scale[tid] = sum == 0.f ? 0.f : 1.0f / sum;
+    }
+    __syncthreads();
+    const uint32_t in = tid % per, d4 = tid / per, row = row_first + in;
+    if (row >= s.rows) return;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (uint32_t i = 0; i < s.sharers; ++i) {
+        const float f = weight[i][in];
+        const float4 x = reinterpret_cast<const float4 *>(slot_of(i) + 2 * BR)[d4 * BR + row];
+        if (f != 0.f) {
+            o.x = fmaf(f, x.x, o.x);
+            o.y = fmaf(f, x.y, o.y);
+            o.z = fmaf(f, x.z, o.z);
+            o.w = fmaf(f, x.w, o.w);
+        }
+    }
+    const uint32_t r = s.row0 + row;
+    const float f = scale[in];
+    T *out = (T *)a.op.out + (uint64_t)(q.q0 + r / group) * a.op.out_token_stride +
+             (uint64_t)(s.head * group + r % group) * a.op.out_head_stride + d4 * 4;
+    *reinterpret_cast<uint2 *>(out) = make_uint2(pack_pair<T>(o.x * f, o.y * f), pack_pair<T>(o.z * f, o.w * f));
+}
+
+template <typename T, int D, int NT>
+ctox_status rows_launch(ctox_ctx *ctx, AttnArgs a) {
+    using R = Rows<D, NT>;
+    a.shape.block_rows = R::BR;
+    a.shape.half_rows = R::BR;
+    a.shape.key_tile = R::KT;
+    a.box = R::KT;
+    while (a.op.kv.page_tokens % a.box) a.box /= 2;
+    CUtensorMap mk, mv;
+    EX(cache_map(ctx, &mk, a.op, a.op.kv.k, a.box, D / 64));
+    EX(cache_map(ctx, &mv, a.op, a.op.kv.v, a.box, D / 64));
+    const size_t smem = R::smem(a.op.n_requests);
+    auto kernel = k_attention_rows<T, D, NT>;
+    CTOX_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const uint32_t grid = (uint32_t)ctx->sm_count;
+    CTOX_CUDA(ctx, launch_pdl(kernel, dim3(grid), dim3(R::NW * 32 + 32), smem, ctx->stream, mk, mv, a, ctx->dev_error));
+    // the longest unit that there can be: where not even that is cut, there is nothing to merge
+    const uint32_t most = a.shape.overhead + (a.op.max_kv_tokens + R::KT - 1) / R::KT;
+    if (keeps_whole(most, a.least)) return CTOX_OK;
+    const uint32_t per = 4 * kMergeThreads / D;
+    CTOX_CUDA(ctx, launch_pdl(k_attention_merge<T>, dim3(grid, (R::BR + per - 1) / per), dim3(kMergeThreads), 0, ctx->stream, a));
+    return CTOX_OK;
+}
+template <typename T, int D>
+ctox_status rows_launch(ctox_ctx *ctx, const AttnArgs &a) {
+    const uint64_t rows = (uint64_t)a.op.max_new_tokens * a.shape.group;
+    return rows <= 8 ? rows_launch<T, D, 1>(ctx, a) : rows_launch<T, D, 2>(ctx, a);
+}
+template <typename T>
+ctox_status rows_launch(ctox_ctx *ctx, const AttnArgs &a) {
+    return a.op.dim == 64 ? rows_launch<T, 64>(ctx, a) : a.op.dim == 128 ? rows_launch<T, 128>(ctx, a) : rows_launch<T, 256>(ctx, a);
+}
+
+}  // namespace
+
+ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attention_op &op, const void *base, uint32_t box, uint32_t chunks) {
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return (Encode)fn;
+    }();
+    if (!encode) return fail(ctx, CTOX_UNSUPPORTED_OPERATION, "cuTensorMapEncodeTiled is not available");
+    const ctox_paged_kv &kv = op.kv;
+    // one axis runs over pages and heads
+    const uint64_t step = op.kv_heads > 1 ? kv.head_stride : kv.page_stride, per_page = op.kv_heads > 1 ? kv.page_stride / kv.head_stride : 1;
+    const cuuint64_t dims[5] = {64, 8, op.dim / 64, kv.page_tokens / 8, (uint64_t)(kv.n_pages - 1) * per_page + op.kv_heads};
+    const cuuint64_t strides[4] = {kv.token_stride * 2, 128, kv.token_stride * 16, step * 2};
+    const cuuint32_t boxes[5] = {64, 8, chunks, box / 8, 1}, each[5] = {1, 1, 1, 1, 1};
+    const CUresult r = encode(map, kv.dtype == CTOX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                              const_cast<void *>(base), dims, strides, boxes, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(ctx, CTOX_SHAPE, "paged attention: a cache of %u pages with strides %llu, %llu, %llu has no tensor map (error %d)", kv.n_pages,
+                    (unsigned long long)kv.page_stride, (unsigned long long)kv.token_stride, (unsigned long long)kv.head_stride, (int)r);
+    return CTOX_OK;
+}
+
+ctox_status launch_attention_rows(ctox_ctx *ctx, const AttnArgs &a) {
+    return a.op.kv.dtype == CTOX_BF16 ? rows_launch<__nv_bfloat16>(ctx, a) : rows_launch<__half>(ctx, a);
+}
+
+static ctox_status check_heads(ctox_ctx *ctx, const ctox_paged_attention_op *op) {
+    const char *what = "paged attention";
+    if (!op) return fail(ctx, CTOX_SHAPE, "%s: no operation", what);
+    EX(check_dim(ctx, op->dim, what));
+    if (!op->heads || !op->kv_heads || op->heads > 65535 || op->heads % op->kv_heads || op->heads / op->kv_heads > 128)
+        return fail(ctx, CTOX_SHAPE, "%s: %u query heads over %u KV heads (a multiple, up to 128 times)", what, op->heads, op->kv_heads);
+    return CTOX_OK;
+}
+static uint64_t workspace_bytes(const ctox_ctx *ctx, const ctox_paged_attention_op &op) {
+    return (uint64_t)ctx->sm_count * (2 * slot_floats(16, op.dim) * 4 + sizeof(Shared)) + 256;
+}
+
+}  // namespace paged
+}  // namespace ctox
+
+using namespace ctox;
+using namespace ctox::paged;
+
+extern "C" {
+
+ctox_status ctox_paged_attention_workspace(ctox_ctx *ctx, const ctox_paged_attention_op *op, uint64_t *bytes) {
+    EX(check_heads(ctx, op));
+    if (!bytes) return fail(ctx, CTOX_SHAPE, "paged attention: no place for the answer");
+    if (!ctx) return fail(ctx, CTOX_INVALID_STATE, "paged attention: no context");
+    *bytes = workspace_bytes(ctx, *op);
+    return CTOX_OK;
+}
+
+ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *op) {
+    const char *what = "paged attention";
+    EX(check_heads(ctx, op));
+    EX(check_kv(ctx, op->kv, op->kv_heads, what));
+    if (!op->n_requests || op->n_requests > CTOX_MAX_BATCH)
+        return fail(ctx, CTOX_SHAPE, "%s: %u requests (1 to %u)", what, op->n_requests, CTOX_MAX_BATCH);
+    if (op->n_tokens > 0x7fffffffu || op->max_new_tokens > 0x7fffffffu || op->max_kv_tokens > 0x7fffffffu ||
+        (uint64_t)op->max_new_tokens * op->heads > 0x7fffffffull)
+        return fail(ctx, CTOX_SHAPE, "%s: %u tokens, up to %u new ones and %u in the cache", what, op->n_tokens, op->max_new_tokens,
+                    op->max_kv_tokens);
+    if (op->causal > 1 || (op->window && !op->causal))
+        return fail(ctx, CTOX_UNSUPPORTED_OPERATION, "%s: causal %u with a window of %u", what, op->causal, op->window);
+    if (!std::isfinite(op->scale) || op->scale <= 0) return fail(ctx, CTOX_SHAPE, "%s: scale %g", what, op->scale);
+    if (!op->query_offsets || !op->kv_lens || !op->block_table) return fail(ctx, CTOX_SHAPE, "%s: null device pointer", what);
+    if (!op->table_rows || !op->max_pages || op->table_stride < op->max_pages || (uint64_t)op->max_pages * op->kv.page_tokens > 0x7fffffffull)
+        return fail(ctx, CTOX_SHAPE, "%s: block table of %u rows, %u pages each, stride %llu", what, op->table_rows, op->max_pages,
+                    (unsigned long long)op->table_stride);
+    if (op->n_tokens && (!op->q || !op->out || !aligned16(op->q) || !aligned16(op->out) || op->q_token_stride % 8 || op->q_head_stride % 8 ||
+                         op->out_token_stride % 8 || op->out_head_stride % 8))
+        return fail(ctx, CTOX_SHAPE, "%s: q and out want 16-byte aligned matrices and strides of multiples of 8", what);
+    if (!ctx) return fail(ctx, CTOX_INVALID_STATE, "%s: no context", what);
+    if (!op->workspace || !aligned16(op->workspace) || op->workspace_bytes < workspace_bytes(ctx, *op))
+        return fail(ctx, CTOX_SHAPE, "%s: workspace of %llu bytes, %llu wanted, aligned to 16", what, (unsigned long long)op->workspace_bytes,
+                    (unsigned long long)workspace_bytes(ctx, *op));
+    if (ctx->sm_count > (int)kMostCtas) return fail(ctx, CTOX_UNSUPPORTED_OPERATION, "%s: %d SMs", what, ctx->sm_count);
+    if (!op->n_tokens || !op->max_new_tokens) return CTOX_OK;
+    AttnArgs a = {};
+    a.op = *op;
+    a.shape.kv_heads = op->kv_heads;
+    a.shape.group = op->heads / op->kv_heads;
+    a.shape.causal = op->causal;
+    a.shape.window = op->window;
+    a.shape.least_rows = 1;
+    a.shape.most_rows = 0x7fffffffu;
+    a.shape.overhead = 2;
+    a.least = 4;
+    a.pages_per_step = op->kv_heads > 1 ? (uint32_t)(op->kv.page_stride / op->kv.head_stride) : 1;
+    a.c = op->scale * 1.4426950408889634f;
+    a.shared = (Shared *)op->workspace;
+    a.partial = (float *)((uint8_t *)op->workspace + ((ctx->sm_count * sizeof(Shared) + 255) & ~255ull));
+    const DeviceGuard guard(ctx->device);
+    CTOX_CUDA(ctx, guard.error());
+    return launch_attention_rows(ctx, a);
+}
+
+}  // extern "C"

@@ -1,0 +1,104 @@
+// Attention over a paged K/V cache: what its kernels share (dealing of the work, partial results, descriptors of the cache).
+#pragma once
+
+#include "paged.cuh"
+#include "umma.cuh"
+
+namespace ctox {
+namespace paged {
+
+// A unit that several CTAs share: the first of them writes this down, the merge reads it.
+struct Shared {
+    uint32_t sharers;  // 0: none begins here
+    uint32_t request, head, row0, rows;
+};
+
+struct AttnArgs {
+    ctox_paged_attention_op op;
+    Shape shape;
+    uint32_t least;          // cost below which a piece of the work is not worth a CTA
+    uint32_t box;            // tokens of a copy: what a page and a key tile are both multiples of
+    uint32_t pages_per_step; // page_stride / head_stride where there are several heads, else 1
+    float c;                 // scale * log2(e)
+    float *partial;          // per CTA two slots: a unit that began before it, one that goes on behind it
+    Shared *shared;          // per CTA
+};
+// Slot layout: running maximum (times log2 e) and sum of each row, then the output, four dimensions of all rows at a time.
+__host__ __device__ inline uint64_t slot_floats(uint32_t rows, uint32_t dim) { return (uint64_t)rows * (dim + 2); }
+
+#ifdef __CUDACC__
+// Request i; false, and its device error, where its numbers lie outside their bounds.
+__device__ __forceinline__ bool read_request(const AttnArgs &a, uint32_t i, Request &q) {
+    const ctox_paged_attention_op &op = a.op;
+    const int32_t q0 = op.query_offsets[i], q1 = op.query_offsets[i + 1], kv = op.kv_lens[i];
+    const int32_t row = op.rows ? op.rows[i] : (int32_t)i;
+    q.q0 = (uint32_t)q0;
+    q.rows_new = (uint32_t)(q1 - q0);
+    q.kv = (uint32_t)kv;
+    return q0 >= 0 && q1 >= q0 && (uint32_t)q1 <= op.n_tokens && q.rows_new <= op.max_new_tokens && kv >= 0 && q.kv <= op.max_kv_tokens &&
+           (uint64_t)q.kv <= (uint64_t)op.max_pages * op.kv.page_tokens && row >= 0 && (uint32_t)row < op.table_rows;
+}
+__device__ __forceinline__ const int32_t *table_row(const AttnArgs &a, uint32_t i) {
+    return a.op.block_table + (uint64_t)(a.op.rows ? a.op.rows[i] : (int32_t)i) * a.op.table_stride;
+}
+
+// Line places of all requests: at[0 .. n], by the whole block. Returns the line's length.
+__device__ __forceinline__ uint64_t lay_line(const AttnArgs &a, unsigned long long *at, unsigned long long *scan, int32_t *error_word) {
+    const uint32_t n = a.op.n_requests, per = (n + blockDim.x - 1) / blockDim.x, r0 = threadIdx.x * per;
+    unsigned long long mine = 0;
+    for (uint32_t r = r0; r < r0 + per && r < n; ++r) {
+        Request q;
+        unsigned long long cost = 0;
+        if (read_request(a, r, q)) {
+            const uint32_t blocks = blocks_of(a.shape, q);
+            for (uint32_t b = 0; b < blocks; ++b) cost += unit_of(a.shape, q, b).cost;
+        } else if (blockIdx.x == 0) {
+            bad_index(error_word);
+        }
+        at[r + 1] = cost * a.shape.kv_heads;
+        mine += at[r + 1];
+    }
+    unsigned long long before = block_scan<unsigned long long>(mine, scan) - mine;
+    for (uint32_t r = r0; r < r0 + per && r < n; ++r) at[r + 1] = before += at[r + 1];
+    if (threadIdx.x == 0) at[0] = 0;
+    __syncthreads();
+    return at[n];
+}
+
+// The line for the walks of paged_plan.cuh.
+struct Line {
+    const AttnArgs &a;
+    const unsigned long long *places;
+    uint32_t n;
+    __device__ __forceinline__ uint64_t at(uint32_t i) const { return places[i]; }
+    __device__ __forceinline__ void request(uint32_t i, Request &q) const { read_request(a, i, q); }
+};
+
+// Page of a token for the copies; false (and the device error) where the table's entry is none.
+__device__ __forceinline__ bool page_at(const AttnArgs &a, const int32_t *table, uint32_t token, int32_t &page, int32_t *error_word) {
+    page = table[token / a.op.kv.page_tokens];
+    if (page >= 0 && (uint32_t)page < a.op.kv.n_pages) return true;
+    bad_index(error_word);
+    return false;
+}
+// Copies `box` tokens of one head: columns [chunk * 64, ...) as wide as the map's box, groups of eight tokens.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, uint32_t bar, int chunk, int group, int step) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(0), "r"(chunk), "r"(group), "r"(step)
+        : "memory");
+}
+__device__ __forceinline__ int box_step(const AttnArgs &a, int32_t page, uint32_t head) {
+    return (int)((uint32_t)page * a.pages_per_step + (a.op.kv_heads > 1 ? head : 0));
+}
+#endif
+
+// The cache as tensor maps: boxes of `box` tokens by chunks * 64 dimensions of one head. In shared memory eight tokens are
+// together, 128 bytes each, swizzled, chunk after chunk.
+ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attention_op &op, const void *base, uint32_t box, uint32_t chunks);
+
+// Requests with few rows (paged_attention.cu) and with many (paged_attention_tile.cu).
+ctox_status launch_attention_rows(ctox_ctx *ctx, const AttnArgs &a);
+
+}  // namespace paged
+}  // namespace ctox

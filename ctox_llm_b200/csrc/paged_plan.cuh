@@ -1,0 +1,205 @@
+// How the work of a batch's attention is dealt to CTAs. Plain integer arithmetic, also compiled for the host.
+//
+// The rows of a request and KV head (its new tokens times the query heads that share the head) are cut into blocks; a
+// block against the keys that it sees is a unit. Units stand one after the other on a line, each as long as its key tiles
+// plus a constant for what a unit costs besides. The line is cut into one equal piece per CTA: the lengths alone decide, no
+// CTA waits for another, and no batch leaves an SM idle for more than a tile. A unit that a cut crosses is
+// finished by the merge (paged_attention.cu). Cuts within short units move to the nearer end of the unit.
+#pragma once
+
+#include <cstdint>
+
+#ifdef __CUDACC__
+#define CTOX_HD __host__ __device__ __forceinline__
+#else
+#define CTOX_HD inline
+#endif
+
+namespace ctox {
+namespace paged {
+
+struct Request {
+    uint32_t q0, rows_new, kv;  // first row of q, new tokens, tokens in the cache
+};
+
+struct Shape {
+    uint32_t kv_heads, group;        // query heads per KV head
+    uint32_t block_rows, key_tile;   // of a unit, of a key tile
+    uint32_t half_rows;              // up to that many rows in a block a tile costs 1, else 2
+    uint32_t overhead;               // of a unit, in tiles
+    uint32_t least_rows, most_rows;  // requests with other numbers of rows (tokens x group) are not this kernel's
+    uint32_t causal, window;
+};
+
+// The keys that the rows [row0, row1) of a request see between them.
+CTOX_HD void key_range(const Shape &s, const Request &q, uint32_t row0, uint32_t row1, uint32_t &lo, uint32_t &hi) {
+    lo = 0;
+    hi = q.kv;
+    if (!s.causal) return;
+    const int64_t base = (int64_t)q.kv - q.rows_new;  // keys before the first new one
+    const int64_t first = base + row0 / s.group, last = base + (row1 - 1) / s.group;
+    if (last + 1 < (int64_t)hi) hi = last + 1 > 0 ? (uint32_t)(last + 1) : 0;
+    if (s.window && first + 1 > (int64_t)s.window) lo = (uint32_t)(first + 1 - s.window);
+    if (lo > hi) lo = hi;
+}
+CTOX_HD uint32_t rows_of(const Shape &s, const Request &q) {
+    const uint64_t rows = (uint64_t)q.rows_new * s.group;
+    return rows >= s.least_rows && rows <= s.most_rows ? (uint32_t)rows : 0;
+}
+CTOX_HD uint32_t blocks_of(const Shape &s, const Request &q) { return (rows_of(s, q) + s.block_rows - 1) / s.block_rows; }
+
+struct Unit {
+    uint32_t row0, rows;   // of the request's rows
+    uint32_t lo, hi;       // keys
+    uint32_t tile0, tiles; // first key tile, number of them
+    uint32_t weight;       // cost of a tile
+    uint32_t cost;
+};
+CTOX_HD Unit unit_of(const Shape &s, const Request &q, uint32_t block) {
+    Unit u;
+    const uint32_t rows = rows_of(s, q);
+    u.row0 = block * s.block_rows;
+    u.rows = rows - u.row0 < s.block_rows ? rows - u.row0 : s.block_rows;
+    key_range(s, q, u.row0, u.row0 + u.rows, u.lo, u.hi);
+    u.tile0 = u.lo / s.key_tile;
+    u.tiles = u.hi > u.lo ? (u.hi + s.key_tile - 1) / s.key_tile - u.tile0 : 0;
+    u.weight = u.rows > s.half_rows ? 2 : 1;
+    u.cost = s.overhead + u.tiles * u.weight;
+    return u;
+}
+
+// Cuts. `total` is the line's length, `ctas` the most pieces; pieces shorter than `least` are not worth a CTA.
+CTOX_HD uint32_t pieces_of(uint64_t total, uint32_t ctas, uint32_t least) {
+    const uint64_t n = total / least;
+    return n < 1 ? 1 : n < ctas ? (uint32_t)n : ctas;
+}
+CTOX_HD uint64_t raw_cut(uint64_t total, uint32_t pieces, uint32_t i) { return total * i / pieces; }
+// A unit this short is not cut.
+CTOX_HD bool keeps_whole(uint32_t cost, uint32_t least) { return cost < 2 * least; }
+CTOX_HD uint64_t cut_in_unit(uint64_t x, uint64_t start, uint32_t cost, uint32_t least) {
+    return !keeps_whole(cost, least) ? x : 2 * (x - start) <= cost ? start : start + cost;
+}
+// CTAs that share a unit which starts in piece `first` and ends at `end`.
+CTOX_HD uint32_t sharers(uint64_t total, uint32_t pieces, uint32_t first, uint64_t end) {
+    return (uint32_t)((end * pieces + total - 1) / total - 1 - first) + 1;
+}
+// Tiles of a unit before place x of the line.
+CTOX_HD uint32_t tiles_before(const Shape &s, const Unit &u, uint64_t start, uint64_t x) {
+    if (x >= start + u.cost) return u.tiles;
+    if (x <= start + s.overhead) return 0;
+    const uint32_t t = ((uint32_t)(x - start - s.overhead) + u.weight - 1) / u.weight;
+    return t < u.tiles ? t : u.tiles;
+}
+
+// A place on the line and the unit there. Line: n requests, at(i) their places (at(n) the end), request(i, q) their numbers.
+struct Cut {
+    uint64_t x, start;  // start: of the unit
+    uint32_t request, head, block;
+};
+// First block of a request whose unit ends behind `off` (from the start of its head); moves `off` to that unit's start. On the
+// device by a whole warp, 32 blocks at a time: a long prompt has thousands.
+CTOX_HD uint32_t find_block(const Shape &s, const Request &q, uint64_t &off) {
+    const uint32_t blocks = blocks_of(s, q);
+#ifdef __CUDA_ARCH__
+    const uint32_t lane = threadIdx.x & 31;
+    uint64_t begin = 0;
+    for (uint32_t b0 = 0;; b0 += 32) {
+        const uint32_t cost = b0 + lane < blocks ? unit_of(s, q, b0 + lane).cost : 0;
+        unsigned long long upto = cost;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= (uint32_t)o) upto += u;
+        }
+        const uint32_t beyond = __ballot_sync(0xffffffffu, off < begin + upto);
+        if (beyond || b0 + 32 >= blocks) {
+            const uint32_t l = beyond ? __ffs(beyond) - 1 : (blocks - 1) & 31;
+            off = begin + __shfl_sync(0xffffffffu, upto - cost, l);
+            return b0 + l;
+        }
+        begin += __shfl_sync(0xffffffffu, upto, 31);
+    }
+#else
+    uint64_t begin = 0;
+    for (uint32_t b = 0;; ++b) {
+        const uint32_t cost = unit_of(s, q, b).cost;
+        if (off < begin + cost || b + 1 == blocks) {
+            off = begin;
+            return b;
+        }
+        begin += cost;
+    }
+#endif
+}
+// The unit at place x, which lies before the line's end.
+template <class Line>
+CTOX_HD Cut locate(const Shape &s, const Line &line, uint64_t x) {
+    // the last request that begins at or before x has something there: those without any work begin where the next one does
+    uint32_t lo = 0, hi = line.n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (line.at(mid) <= x)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    Cut c;
+    c.x = x;
+    c.request = lo;
+    Request q;
+    line.request(lo, q);
+    const uint64_t per_head = (line.at(lo + 1) - line.at(lo)) / s.kv_heads, in = x - line.at(lo);
+    c.head = (uint32_t)(in / per_head);
+    uint64_t off = in - c.head * per_head;
+    c.block = find_block(s, q, off);
+    c.start = line.at(lo) + c.head * per_head + off;
+    return c;
+}
+// Cut i of `pieces`, moved out of a unit that is too short to be cut.
+template <class Line>
+CTOX_HD Cut cut_at(const Shape &s, const Line &line, uint64_t total, uint32_t pieces, uint32_t i, uint32_t least) {
+    const uint64_t x = raw_cut(total, pieces, i);
+    if (x >= total) return Cut{total, total, 0, 0, 0};
+    Cut c = locate(s, line, x);
+    Request q;
+    line.request(c.request, q);
+    const uint32_t cost = unit_of(s, q, c.block).cost;
+    c.x = cut_in_unit(x, c.start, cost, least);
+    if (c.x < c.start + cost) return c;
+    return c.x >= total ? Cut{total, total, 0, 0, 0} : locate(s, line, c.x);
+}
+
+// A CTA's share of the line, unit by unit.
+struct Walk {
+    Cut at;
+    uint64_t end;
+    Request q;
+    Unit u;
+    uint32_t tile0, tile1;  // of the unit, in this CTA
+    bool begins, ends;      // the unit, in this CTA
+};
+template <class Line>
+CTOX_HD bool walk_unit(const Shape &s, const Line &line, Walk &w) {
+    if (w.at.x >= w.end) return false;
+    line.request(w.at.request, w.q);
+    w.u = unit_of(s, w.q, w.at.block);
+    w.tile0 = tiles_before(s, w.u, w.at.start, w.at.x);
+    w.tile1 = tiles_before(s, w.u, w.at.start, w.end);
+    w.begins = w.at.x == w.at.start;
+    w.ends = w.end >= w.at.start + w.u.cost;
+    return true;
+}
+template <class Line>
+CTOX_HD void walk_on(const Shape &s, const Line &line, Walk &w) {
+    w.at.x = w.at.start = w.at.start + w.u.cost;
+    if (++w.at.block < blocks_of(s, w.q)) return;
+    w.at.block = 0;
+    if (++w.at.head < s.kv_heads) return;
+    w.at.head = 0;
+    if (w.at.x >= w.end) return;
+    do ++w.at.request;
+    while (line.at(w.at.request + 1) == line.at(w.at.request));  // x lies before the line's end: one with work follows
+}
+
+}  // namespace paged
+}  // namespace ctox

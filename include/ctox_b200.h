@@ -298,6 +298,140 @@ ctox_status ctox_gated_delta_prepare(ctox_ctx *ctx, const float *a, const float 
                                      const float *a_log, const float *dt_bias, float *log_decay,
                                      float *beta, uint32_t tokens, uint32_t heads);
 
+/* ---- a K/V cache in pages that many requests share (no counterpart in the reference, whose paged cache
+ * holds one session: kv_cache.rs:76-480) ----
+ * The three steps of serving a batch: ctox_page_slots finds pages and slots for the new tokens of every
+ * request, ctox_rope_append rotates a layer's queries and keys and stores keys and values in those slots,
+ * ctox_paged_attention lets the queries attend to what their request has in the cache. Lengths, tables and
+ * slots stay in device memory and are read by the kernels, so a step can be captured into a CUDA graph and
+ * replayed with other lengths. All pointers are device memory and 4-byte aligned (16 where noted); everything
+ * is enqueued on the context's stream, nothing is allocated and nothing is kept between calls. An operation
+ * is checked before anything is enqueued (CTOX_SHAPE and so on; `ctx` NULL: after the check, CTOX_INVALID_STATE).
+ * What only the device can see (an index out of range, a length above its bound) sets the device error word;
+ * the access is left out, and what the call wrote for that request is undefined.
+ * Batch index: the i-th request of the call. `rows` (may be NULL: row i) names the row of the block table that
+ * belongs to request i, different for different requests; a server keeps rows for as long as requests live. */
+#define CTOX_MAX_BATCH 2048
+
+/* Key and value of token t, KV head h: element page * page_stride + (t % page_tokens) * token_stride +
+ * h * head_stride of k and v, where page = block_table[row * table_stride + t / page_tokens] and the head's
+ * `dim` elements are neighbours. Strides in elements, multiples of 8; k and v aligned to 16 bytes.
+ * page_tokens is a multiple of 16; page_stride is a multiple of head_stride where there are several heads.
+ * Both [page][token][head][dim] (the executor's order) and [page][head][token][dim] are such layouts, also
+ * with a token's keys and values side by side. dtype: CTOX_BF16 or CTOX_F16. */
+typedef struct {
+    void *k, *v;
+    uint32_t dtype, page_tokens, n_pages;
+    uint64_t page_stride, token_stride, head_stride;
+} ctox_paged_kv;
+
+/* Request i has kv_lens_in[i] tokens in the cache and gets new_tokens[i] (zero allowed). Pages that it needs
+ * beyond those it holds come from the stack free_pages[0 .. count), the top first, request by request; they
+ * are entered into its row of the block table. Written: query_offsets[0 .. n_requests] (the new tokens of
+ * request i are tokens query_offsets[i] .. query_offsets[i + 1] - 1 of the batch), and for each token its slot
+ * (page * page_tokens + place in the page), position and request; tokens behind the last one, up to n_tokens,
+ * get slot -1, position 0 and request -1. kv_lens_out[i] = kv_lens_in[i] + new_tokens[i]; free_count_out =
+ * pages left. The *_out arrays may be the *_in arrays, or others, which leaves those as they were.
+ * status[0]: pages taken; status[1]: 0, or CTOX_PAGES_* bits. With any bit set nothing is taken: lengths, count
+ * and table stay, all query_offsets are 0 and all slots -1. */
+enum {
+    CTOX_PAGES_NONE_FREE = 1,  /* the stack holds fewer pages than are needed */
+    CTOX_PAGES_ROW_FULL = 2,   /* a request would need more than max_pages pages */
+    CTOX_PAGES_TOO_MANY = 4,   /* more new tokens than n_tokens (release: more pages than n_pages) */
+    CTOX_PAGES_BAD_INPUT = 8   /* a negative length or count, or a row outside the table */
+};
+typedef struct {
+    uint32_t n_requests, page_tokens, n_pages, table_rows, max_pages, n_tokens;
+    const int32_t *new_tokens, *rows, *kv_lens_in;
+    int32_t *kv_lens_out;
+    int32_t *block_table;
+    uint64_t table_stride;
+    const int32_t *free_pages;
+    const int32_t *free_count_in;
+    int32_t *free_count_out;
+    int32_t *query_offsets, *slots, *positions, *requests; /* requests may be NULL */
+    int32_t *status;
+} ctox_page_slots_op;
+ctox_status ctox_page_slots(ctox_ctx *ctx, const ctox_page_slots_op *op);
+
+/* The way back: the pages of finished requests (kv_lens[i] tokens each, zero allowed) go onto the stack in
+ * order, their table entries become -1. status as above. */
+typedef struct {
+    uint32_t n_requests, page_tokens, n_pages, table_rows, max_pages;
+    const int32_t *rows, *kv_lens;
+    int32_t *block_table;
+    uint64_t table_stride;
+    int32_t *free_pages;
+    const int32_t *free_count_in;
+    int32_t *free_count_out;
+    int32_t *status;
+} ctox_page_release_op;
+ctox_status ctox_page_release(ctox_ctx *ctx, const ctox_page_release_op *op);
+
+/* Queries, keys and values of one layer on their way from the projections: with norm weights an RMS norm
+ * over each head, x / sqrt(mean x^2 + norm_eps) * (norm_offset + w) (norm_offset 1 with weights stored around
+ * zero, reference.rs:38-64); then the first rot_dim dimensions of every query and key head are rotated, pair i by
+ * positions[axis[i]][token] * rope_base^(-2i / rot_dim): one axis for text, three (time, height, width) for
+ * images and video. CTOX_ROPE_HALF pairs i with i + rot_dim / 2 (reference.rs:115-155), CTOX_ROPE_ADJACENT 2i with
+ * 2i + 1. Angles are formed in 64 bits, everything else in 32, and rounded once to kv.dtype, the type of q_out.
+ * Keys and values go to slots[token] (negative: not stored); what two tokens with one slot leave there is
+ * undefined. q NULL: keys and values only; k and v NULL: queries only. dim 64, 128 or 256; all strides are multiples of
+ * 8 elements, all matrices and norm weights aligned to 16 bytes. source_dtype: CTOX_F32, CTOX_BF16 or CTOX_F16. q_out must not overlap
+ * the sources. */
+enum { CTOX_ROPE_HALF = 0, CTOX_ROPE_ADJACENT = 1 };
+typedef struct {
+    uint32_t tokens, heads, kv_heads, dim, rot_dim, axes, pairing, source_dtype;
+    double rope_base;
+    uint8_t axis[128]; /* of each pair; below `axes` */
+    const int32_t *positions;
+    uint64_t position_stride; /* from one axis to the next */
+    const void *q, *k, *v;
+    uint64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const float *q_norm, *k_norm; /* may be NULL */
+    float norm_offset, norm_eps;
+    void *q_out;
+    uint64_t q_out_token_stride, q_out_head_stride;
+    const int32_t *slots;
+    ctox_paged_kv kv;
+} ctox_rope_append_op;
+ctox_status ctox_rope_append(ctox_ctx *ctx, const ctox_rope_append_op *op);
+
+/* Attention of the batch's tokens over the cache, which holds their own keys and values already. Request i has
+ * kv_lens[i] tokens there and rows query_offsets[i] .. query_offsets[i + 1] - 1 of q and out; query head h reads
+ * KV head h / (heads / kv_heads). With `causal` its j-th row sees the keys 0 .. kv_lens[i] - new + j (new its number of
+ * rows), with a window only the last `window` of them; without, every row sees all keys (cross attention to states of
+ * another length). out = sum_t w_t v_t / sum_t w_t, w_t = exp(scale q . k_t); with sinks the denominator has one more term
+ * exp(sinks[h]). A row that sees nothing is zero. Rows of no request stay as they were. Keys and values that no row
+ * of a request sees (other pages, the rest of a last page, what left every window) are not used, whatever
+ * they hold; a value that is not finite reaches the rows that see it and may reach neighbouring rows of its request.
+ * q, out and the cache have the type kv.dtype; scores, weights' sums and the output before its rounding are in 32 bits,
+ * weights enter the product with the values in kv.dtype. dim 64, 128 or 256; heads / kv_heads at most 128;
+ * strides multiples of 8 elements, q and out aligned to 16 bytes; out must not overlap q.
+ * max_new_tokens and max_kv_tokens are upper bounds of a request's rows and length, known on the host: they
+ * choose the kernels. Longer requests set the device error word and are left out.
+ * workspace: ctox_paged_attention_workspace() bytes, aligned to 16; what it holds does not matter and is not
+ * kept. Calls that may run at the same time (two graphs on two streams) need one each. */
+typedef struct {
+    uint32_t n_requests, n_tokens, max_new_tokens, max_kv_tokens;
+    uint32_t heads, kv_heads, dim, causal, window;
+    float scale;
+    const int32_t *query_offsets, *kv_lens, *rows;
+    const int32_t *block_table;
+    uint32_t table_rows, max_pages;
+    uint64_t table_stride;
+    const float *sinks; /* [heads], may be NULL */
+    const void *q;
+    uint64_t q_token_stride, q_head_stride;
+    void *out;
+    uint64_t out_token_stride, out_head_stride;
+    void *workspace;
+    uint64_t workspace_bytes;
+    ctox_paged_kv kv;
+} ctox_paged_attention_op;
+/* Bytes that any call with the heads, kv_heads and dim of `op` needs, whatever its lengths. */
+ctox_status ctox_paged_attention_workspace(ctox_ctx *ctx, const ctox_paged_attention_op *op, uint64_t *bytes);
+ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *op);
+
 /* ---- selection (sampler.rs:65-144, engine.rs:203-217,906-963; CUDA candidate
  * backend/cuda_runtime.rs:2376-2917: prepare_argmax_f32 / dispatch_argmax_f32_device,
  * prepare_mtp_compact_result / enqueue_mtp_accept_from_device_drafts /

@@ -1,0 +1,265 @@
+"""Attention over a paged cache against the plain form in 64 bits: sizes around tiles and pages, layouts, masks, shared work."""
+import pytest
+import torch
+
+import ctox_llm_b200 as ctox
+from paged_util import DTYPE, Cache, attention64, attention_op, attention_tolerance, near
+
+pytestmark = pytest.mark.gpu
+N = ctox.native
+
+
+@pytest.fixture(scope="module")
+def be():
+    b = ctox.B200Backend(0, stream=1)  # torch's default stream
+    yield b
+    b.close()
+
+
+def queries(cache, heads, new, seed=5, std=1.5, pad=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(sum(new) + pad, heads, cache.dim, generator=g, device="cuda") * std).to(DTYPE[cache.dtype][0])
+
+
+def check(be, cache, heads, new, seed=5, pad=0, causal=1, window=0, sinks=None, **more):
+    q = queries(cache, heads, new, seed, pad=pad)
+    out = torch.full_like(q, 7.0)
+    op, keep = attention_op(be, cache, q, out, new, causal=causal, window=window, sinks=sinks, **more)
+    be.paged_attention(op)
+    torch.cuda.synchronize()
+    assert be.device_error() == 0
+    T = sum(new)
+    assert (out[T:] == 7.0).all()  # rows of no request stay
+    want, size = attention64(cache, q[:T], new, bool(causal), window, sinks=sinks)
+    assert near(out[:T], want, attention_tolerance(cache.dtype, want, size, max(cache.lens, default=0)))
+    return out
+
+
+HEADS = [(8, 2, 128), (24, 4, 256), (4, 4, 64), (16, 1, 128), (5, 5, 256), (12, 2, 64), (9, 3, 128)]
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_single_tokens_of_many_lengths(be, heads, kv_heads, dim, dtype):
+    lens = [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 200, 511, 640, 1000, 3001]
+    check(be, Cache(lens, kv_heads, dim, 16, dtype), heads, [1] * len(lens))
+
+
+@pytest.mark.parametrize("page", [16, 32, 48, 64, 80, 128, 256])
+@pytest.mark.parametrize("layout", ["nhd", "hnd", "both"])
+def test_pages_and_layouts(be, page, layout):
+    check(be, Cache([5, 130, 777, 1024], 2, 128, page, "bf16", layout), 8, [1, 3, 2, 1])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("new,context", [([2], 0), ([4], 2000), ([5, 1, 7], 33), ([16], 300), ([33, 1, 64], 100), ([200], 0), ([131], 700)])
+def test_several_new_tokens(be, heads, kv_heads, dim, new, context):
+    check(be, Cache([context + m for m in new], kv_heads, dim, 16, "bf16", seed=3), heads, new)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_one_long_context_is_shared_by_all_ctas(be, dim):
+    for heads, kv_heads, new in ((8, 1, 1), (24, 4, 4), (6, 1, 40)):
+        check(be, Cache([20011], kv_heads, dim, 16, "bf16"), heads, [new])
+
+
+@pytest.mark.parametrize("window", [1, 2, 15, 64, 100, 129, 1000])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (6, 1, 256), (4, 4, 64)])
+def test_windows(be, window, heads, kv_heads, dim):
+    check(be, Cache([1, 70, 500, 1500, 300], kv_heads, dim, 16, "bf16"), heads, [1, 3, 1, 2, 150], window=window)
+
+
+def test_what_left_every_window_may_be_gone(be):
+    """Pages before the window are given back: their table entries say so, and attention does not look them up."""
+    c = Cache([1000, 777], 2, 128, 16, "bf16")
+    for i, n in enumerate(c.lens):
+        c.table[c.rows_list[i], :(n - 2 - 100) // 16] = -1
+    check(be, c, 8, [2, 1], window=100)
+
+
+def test_sinks(be):
+    for heads, kv_heads, dim in ((8, 2, 128), (6, 1, 256)):
+        sinks = torch.linspace(-8, 12, heads, device="cuda")
+        check(be, Cache([1, 100, 5000], kv_heads, dim, 16, "bf16"), heads, [1, 40, 2], sinks=sinks)
+        check(be, Cache([30, 2000], kv_heads, dim, 16, "f16"), heads, [1, 1], sinks=sinks, window=64)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (5, 1, 256), (4, 4, 64)])
+def test_states_of_another_length(be, heads, kv_heads, dim):
+    """Not causal: every row sees all keys; a request without any gives zeros."""
+    out = check(be, Cache([37, 0, 1500, 128], kv_heads, dim, 16, "bf16"), heads, [50, 3, 1, 260], causal=0)
+    assert (out[50:53] == 0).all()
+
+
+def test_rows_that_see_nothing_are_zero(be):
+    """More rows than tokens in the cache: the first ones lie before its beginning."""
+    for sinks in (None, torch.zeros(8, device="cuda")):
+        for new in ([5, 9], [40, 60]):
+            out = check(be, Cache([2, 3], 2, 128, 16, "bf16"), 8, new, sinks=sinks)
+            assert (out[:new[0] - 2] == 0).all() and (out[new[0]:sum(new) - 3] == 0).all()
+
+
+def test_requests_without_new_tokens_and_rows_behind_the_last(be):
+    check(be, Cache([100, 0, 50, 2000, 17], 2, 128, 16, "bf16"), 8, [1, 0, 0, 2, 0], pad=9)
+    check(be, Cache([100, 0, 50, 2000, 17], 4, 256, 16, "bf16"), 24, [20, 0, 0, 45, 0], pad=9)
+
+
+def test_strided_queries_and_outputs(be):
+    c = Cache([300, 45], 2, 128, 16, "bf16")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for new in ([2, 1], [70, 30]):
+        T = sum(new)
+        wide = torch.randn(T, 8, 2, 128, generator=g, device="cuda").bfloat16()  # queries beside their gates
+        q = wide[:, :, 0]
+        out = torch.full((8, T, 128), 3.0, device="cuda").bfloat16().transpose(0, 1)
+        op, keep = attention_op(be, c, q, out, new)
+        be.paged_attention(op)
+        want, size = attention64(c, q, new)
+        assert near(out, want, attention_tolerance("bf16", want, size, 300))
+
+
+def test_large_scores(be):
+    """Scores in the hundreds: one key takes nearly all weight, and the maximum moves from tile to tile."""
+    c = Cache([900, 1300], 2, 128, 16, "bf16", seed=9)
+    for i in range(2):
+        for t in range(0, c.lens[i], 60):  # keys that grow
+            c.key[i][t] = c.key[i][0] * (1 + t / 100)
+            c.k[c.pages[i][t // 16], t % 16] = c.key[i][t]
+    for new in ([1, 2], [1, 300]):
+        q = queries(c, 8, new, std=8.0)
+        out = torch.empty_like(q)
+        op, keep = attention_op(be, c, q, out, new)
+        be.paged_attention(op)
+        want, size = attention64(c, q, new)
+        # scores up to 8 * 14 * 14 * sqrt(128) or so: 2^11, and each of its 24 additions is off by 2^-23 of it
+        tolerance = attention_tolerance("bf16", want, size, 1300) + 2 * 24 * 2.0 ** (11 - 23) * size
+        assert near(out, want, tolerance)
+
+
+def test_many_requests(be):
+    g = torch.Generator().manual_seed(2)
+    lens = torch.randint(1, 400, (2048,), generator=g).tolist()
+    check(be, Cache(lens, 1, 64, 16, "bf16"), 4, [1] * 2048)
+    new = [1 + (i % 37 == 0) * 50 for i in range(300)]
+    check(be, Cache([lens[i] + m for i, m in enumerate(new)], 2, 128, 16, "f16"), 8, new)
+
+
+def test_bounds_that_are_larger_than_needed(be):
+    """Captured programs name bounds for all of their replays."""
+    check(be, Cache([40, 700], 2, 128, 16, "bf16"), 8, [1, 2], max_new_tokens=200, max_kv_tokens=100000)
+    check(be, Cache([40, 700], 4, 256, 16, "bf16"), 24, [1, 30], max_new_tokens=4000, max_kv_tokens=100000)
+
+
+def test_the_same_bits_every_time(be):
+    c = Cache([3000, 17, 9000], 4, 256, 16, "bf16")
+    for new in ([1, 1, 2], [4, 1, 150]):
+        q = queries(c, 24, new)
+        outs = []
+        for _ in range(5):
+            out = torch.empty_like(q)
+            op, keep = attention_op(be, c, q, out, new)
+            be.paged_attention(op)
+            outs.append(out)
+        assert all(torch.equal(outs[0], o) for o in outs)
+
+
+def test_what_only_the_device_sees(be):
+    """Pages, lengths and offsets out of range: the device error word, and the other requests are served."""
+    def run(new, change, good):
+        c = Cache([100, 200, 40], 2, 128, 16, "bf16")
+        q = queries(c, 8, new)
+        out = torch.full_like(q, 7.0)
+        op, keep = attention_op(be, c, q, out, new)
+        change(c, op, keep)
+        be.paged_attention(op)
+        torch.cuda.synchronize()
+        assert be.device_error() == 4 and be.device_error() == 0
+        want, size = attention64(c, q, new)
+        a, b = sum(new[:good]), sum(new[:good + 1])
+        assert near(out[a:b], want[a:b], attention_tolerance("bf16", want, size, 200)[a:b])
+        return out
+
+    for new in ([1, 2, 1], [40, 30, 33]):
+        run(new, lambda c, op, keep: c.table[c.rows_list[1], 3:5].fill_(c.n_pages), 0)
+        run(new, lambda c, op, keep: c.table[c.rows_list[1], 3:5].fill_(-5), 2)
+        run(new, lambda c, op, keep: keep[1][1:2].fill_(-1), 0)
+        run(new, lambda c, op, keep: keep[1][1:2].fill_(1 << 30), 2)
+        run(new, lambda c, op, keep: c.rows[1:2].fill_(99), 0)
+        run(new, lambda c, op, keep: setattr(op, "max_kv_tokens", 150), 0)
+        out = run(new, lambda c, op, keep: keep[0][3:4].fill_(1 << 20), 1)
+        assert (out[sum(new[:2]):] == 7.0).all()
+
+
+def test_a_workspace_that_is_too_small_is_refused(be):
+    c = Cache([10], 2, 128, 16, "bf16")
+    q = queries(c, 8, [1])
+    op, keep = attention_op(be, c, q, torch.empty_like(q), [1])
+    op.workspace_bytes -= 1
+    with pytest.raises(ctox.CtoxError) as e:
+        be.paged_attention(op)
+    assert e.value.kind == "Shape" and "workspace" in str(e.value)
+    op.workspace, op.workspace_bytes = None, 1 << 40
+    with pytest.raises(ctox.CtoxError):
+        be.paged_attention(op)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [4, 1, 60]])
+def test_a_captured_call_follows_its_lengths(be, new):
+    """One graph, replayed with other lengths, pages and queries."""
+    stream = torch.cuda.Stream()
+    mine = ctox.B200Backend(0, stream=stream.cuda_stream)
+    c = Cache([2000, 300, 900], 2, 128, 16, "bf16")
+    q = queries(c, 8, new)
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    op, keep = attention_op(mine, c, q, out, new, max_kv_tokens=4000)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        mine.paged_attention(op)
+    for lens in ([2000, 300, 900], [new[0], 61, 640]):
+        c.lens = lens
+        c.key, c.value = [k[:n] for k, n in zip(c.key, lens)], [v[:n] for v, n in zip(c.value, lens)]
+        keep[1].copy_(torch.tensor(lens, dtype=torch.int32))
+        q.copy_(queries(c, 8, new, seed=sum(lens)))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, size = attention64(c, q, new)
+        assert near(out, want, attention_tolerance("bf16", want, size, 2000))
+    del graph
+    mine.close()
+
+
+def test_two_streams_at_once(be):
+    """Calls of two contexts that overlap, each with a workspace of its own."""
+    work = []
+    for i in range(2):
+        stream = torch.cuda.Stream()
+        b = ctox.B200Backend(0, stream=stream.cuda_stream)
+        c = Cache([15000 + 100 * i, 200], 4, 256, 16, "bf16", seed=i)
+        q = queries(c, 24, [4, 30], seed=i)
+        out = torch.zeros_like(q)
+        work.append((b, c, q, out, *attention_op(b, c, q, out, [4, 30])))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for b, c, q, out, op, keep in work:
+            b.paged_attention(op)
+    torch.cuda.synchronize()
+    for b, c, q, out, op, keep in work:
+        want, size = attention64(c, q, [4, 30])
+        assert near(out, want, attention_tolerance("bf16", want, size, 16000))
+        b.close()
+
+
+def test_offsets_beyond_32_bits(be):
+    """A cache whose last pages lie behind 2^32 elements."""
+    page, dim = 128, 256
+    n_pages = (1 << 32) // (page * dim) + 40
+    store = torch.empty(n_pages, page, 1, 2 * dim, dtype=torch.bfloat16, device="cuda")  # 17 GB
+    c = Cache([500], 1, dim, page, "bf16", "both")
+    for old, new in zip(c.pages[0], range(n_pages - 4, n_pages)):
+        store[new] = c.store[old]
+    c.table[c.rows_list[0], :4] = torch.arange(n_pages - 4, n_pages, dtype=torch.int32)
+    c.store, c.n_pages = store, n_pages
+    c.k, c.v = store[..., :dim], store[..., dim:]
+    check(be, c, 6, [2])
+    check(be, c, 6, [100])

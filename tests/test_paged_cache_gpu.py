@@ -1,0 +1,360 @@
+"""Pages and slots, rotation and append, and a whole step, against plain forms."""
+import random
+
+import pytest
+import torch
+
+import ctox_llm_b200 as ctox
+from paged_util import DTYPE, Cache, attention64, attention_op, attention_tolerance, near
+
+pytestmark = pytest.mark.gpu
+N = ctox.native
+
+
+@pytest.fixture(scope="module")
+def be():
+    b = ctox.B200Backend(0, stream=1)
+    yield b
+    b.close()
+
+
+class Manager:
+    """The page manager's state in lists, and its device copy."""
+
+    def __init__(self, lens, page, max_pages, n_pages, seed=0, spare_rows=3):
+        rng = random.Random(seed)
+        self.page, self.max_pages, self.n_pages = page, max_pages, n_pages
+        self.rows = rng.sample(range(len(lens) + spare_rows), len(lens))
+        self.table = [[-1] * max_pages for _ in range(len(lens) + spare_rows)]
+        order = rng.sample(range(n_pages), n_pages)
+        self.lens = list(lens)
+        for r, n in zip(self.rows, lens):
+            for j in range(-(-n // page)):
+                self.table[r][j] = order.pop()
+        self.free = order
+
+    def device(self):
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+        d = dict(rows=i32(self.rows), table=i32(self.table), lens=i32(self.lens), count=i32([len(self.free)]))
+        d["free"] = i32(self.free + [-7] * (self.n_pages - len(self.free)))
+        return d
+
+    def take(self, new):
+        """What the operation writes, request by request and token by token."""
+        slots, positions, requests, offsets, start = [], [], [], [0], len(self.free)
+        for i, m in enumerate(new):
+            for t in range(self.lens[i], self.lens[i] + m):
+                if t % self.page == 0:
+                    self.table[self.rows[i]][t // self.page] = self.free.pop()
+                slots.append(self.table[self.rows[i]][t // self.page] * self.page + t % self.page)
+                positions.append(t)
+                requests.append(i)
+            self.lens[i] += m
+            offsets.append(len(slots))
+        return slots, positions, requests, offsets, start - len(self.free)
+
+
+def slots_op(m, d, new, n_tokens, in_place=True, with_rows=True):
+    n = len(new)
+    z = lambda k: torch.full((k,), 99, dtype=torch.int32, device="cuda")
+    o = dict(new=torch.tensor(new, dtype=torch.int32, device="cuda"), offsets=z(n + 1), slots=z(n_tokens + 4), positions=z(n_tokens + 4),
+             requests=z(n_tokens + 4), status=z(2), lens_out=d["lens"] if in_place else z(n), count_out=d["count"] if in_place else z(1))
+    op = ctox.PageSlots(n_requests=n, page_tokens=m.page, n_pages=m.n_pages, table_rows=len(m.table), max_pages=m.max_pages, n_tokens=n_tokens,
+                        new_tokens=o["new"].data_ptr(), rows=d["rows"].data_ptr() if with_rows else None, kv_lens_in=d["lens"].data_ptr(),
+                        kv_lens_out=o["lens_out"].data_ptr(), block_table=d["table"].data_ptr(), table_stride=d["table"].stride(0),
+                        free_pages=d["free"].data_ptr(), free_count_in=d["count"].data_ptr(), free_count_out=o["count_out"].data_ptr(),
+                        query_offsets=o["offsets"].data_ptr(), slots=o["slots"].data_ptr(), positions=o["positions"].data_ptr(),
+                        requests=o["requests"].data_ptr(), status=o["status"].data_ptr())
+    return op, o
+
+
+@pytest.mark.parametrize("lens,new", [([5], [1]), ([0], [1]), ([16], [1]), ([15, 16, 17, 0], [1, 1, 1, 1]), ([0, 3, 40], [100, 0, 7]),
+                                      ([i % 50 for i in range(300)], [1] * 300), ([i for i in range(600)], [(i * 7) % 40 for i in range(600)]),
+                                      ([3] * 2048, [1 + i % 3 for i in range(2048)]), ([33, 1000], [5000, 9001]), ([7, 9], [0, 0])])
+@pytest.mark.parametrize("page", [16, 48])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_slots(be, lens, new, page, in_place):
+    need = [-(-(a + b) // page) for a, b in zip(lens, new)]
+    m = Manager(lens, page, max(need) + 1, sum(need) + 5)
+    d = m.device()
+    before = {k: v.clone() for k, v in d.items()}
+    for _ in range(1 if in_place else 3):  # not in place: the same call again gives the same answer
+        pad = 11
+        op, o = slots_op(m, d, new, sum(new) + pad, in_place)
+        be.page_slots(op)
+    slots, positions, requests, offsets, taken = m.take(new)
+    T = len(slots)
+    assert o["slots"].tolist() == slots + [-1] * pad + [99] * 4
+    assert o["positions"].tolist() == positions + [0] * pad + [99] * 4
+    assert o["requests"].tolist() == requests + [-1] * pad + [99] * 4
+    assert o["offsets"].tolist() == offsets and o["status"].tolist() == [taken, 0]
+    assert o["lens_out"].tolist() == m.lens and o["count_out"].tolist() == [len(m.free)]
+    assert d["table"].tolist() == m.table
+    assert torch.equal(d["free"], before["free"])
+    if not in_place:
+        assert torch.equal(d["lens"], before["lens"]) and torch.equal(d["count"], before["count"])
+    assert be.device_error() == 0
+
+
+def test_slots_that_cannot_be_given_change_nothing(be):
+    cases = [(dict(), [40, 40, 40], N.PAGES_NONE_FREE), (dict(), [1, 200, 1], N.PAGES_ROW_FULL | N.PAGES_NONE_FREE),
+             (dict(room=4), [2, 2, 2], N.PAGES_TOO_MANY), (dict(), [1, -1, 1], N.PAGES_BAD_INPUT), (dict(row=50), [1, 1, 1], N.PAGES_BAD_INPUT),
+             (dict(row=-1), [1, 1, 1], N.PAGES_BAD_INPUT), (dict(len=-4), [1, 1, 1], N.PAGES_BAD_INPUT), (dict(count=-1), [0, 0, 0], N.PAGES_BAD_INPUT),
+             (dict(count=1000), [1, 1, 1], N.PAGES_BAD_INPUT), (dict(), [2 ** 31 - 1] * 3, N.PAGES_ROW_FULL | N.PAGES_NONE_FREE | N.PAGES_TOO_MANY)]
+    for change, new, flags in cases:
+        m = Manager([20, 30, 16], 16, 6, 10)
+        d = m.device()
+        if "row" in change:
+            d["rows"][1] = change["row"]
+        if "len" in change:
+            d["lens"][1] = change["len"]
+        if "count" in change:
+            d["count"][0] = change["count"]
+        before = {k: v.clone() for k, v in d.items()}
+        op, o = slots_op(m, d, new, change.get("room", 300))
+        be.page_slots(op)
+        assert o["status"].tolist() == [0, flags], (change, new, o["status"].tolist())
+        assert all(torch.equal(d[k], before[k]) for k in d)
+        assert o["offsets"].tolist() == [0] * 4 and (o["slots"][:change.get("room", 300)] == -1).all()
+        assert o["lens_out"].tolist() == before["lens"].tolist()
+
+
+def test_a_bad_page_in_the_stack_gives_no_slot(be):
+    m = Manager([16], 16, 4, 5)
+    d = m.device()
+    d["free"][d["count"].item() - 1] = 77
+    op, o = slots_op(m, d, [2], 2)
+    be.page_slots(op)
+    assert o["slots"].tolist()[:2] == [-1, -1] and be.device_error() == 4
+
+
+def release(be, m, d, which):
+    n = len(which)
+    rows = torch.tensor([m.rows[i] for i in which], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([m.lens[i] for i in which], dtype=torch.int32, device="cuda")
+    status = torch.full((2,), 99, dtype=torch.int32, device="cuda")
+    be.page_release(ctox.PageRelease(n_requests=n, page_tokens=m.page, n_pages=m.n_pages, table_rows=len(m.table), max_pages=m.max_pages,
+                                     rows=rows.data_ptr(), kv_lens=lens.data_ptr(), block_table=d["table"].data_ptr(),
+                                     table_stride=d["table"].stride(0), free_pages=d["free"].data_ptr(), free_count_in=d["count"].data_ptr(),
+                                     free_count_out=d["count"].data_ptr(), status=status.data_ptr()))
+    return status.tolist()
+
+
+def test_a_server_takes_and_gives_back(be):
+    """Many steps of requests that come, grow and go: no page is held twice, none is lost."""
+    rng = random.Random(4)
+    m = Manager([0] * 12, 16, 40, 12 * 40)
+    d = m.device()
+    for _ in range(40):
+        new = [rng.choice([0, 1, 1, 1, rng.randint(2, 60)]) for _ in m.lens]
+        new = [b if a + b <= 640 else 0 for a, b in zip(m.lens, new)]
+        op, o = slots_op(m, d, new, sum(new))
+        be.page_slots(op)
+        slots, _, _, _, taken = m.take(new)
+        assert o["slots"].tolist()[:len(slots)] == slots and o["status"].tolist() == [taken, 0]
+        done = rng.sample(range(12), rng.randint(1, 3))
+        given = sum(-(-m.lens[i] // 16) for i in done)
+        assert release(be, m, d, done) == [given, 0]
+        for i in done:
+            for j in range(-(-m.lens[i] // 16)):
+                m.free.append(m.table[m.rows[i]][j])
+                m.table[m.rows[i]][j] = -1
+            m.lens[i] = 0
+            d["lens"][i] = 0
+        assert d["table"].tolist() == m.table and d["count"].item() == len(m.free) and d["free"].tolist()[:len(m.free)] == m.free
+        held = [p for r in m.table for p in r if p >= 0]
+        assert sorted(held + m.free) == list(range(m.n_pages))
+    m.lens[0] = 10 ** 6
+    before = d["count"].item()
+    assert release(be, m, d, [0])[1] & N.PAGES_ROW_FULL and d["count"].item() == before
+
+
+# ---- rotation and append ----
+def rope64(x, weight, offset, eps, positions, axis, base, rot, pairing):
+    """Normed and turned in 64 bits, and the size that rounding scales with."""
+    x = x.double()
+    if weight is not None:
+        x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * (offset + weight.double())
+    if not rot:
+        return x, x.abs()
+    freq = base ** (-torch.arange(0, rot, 2, device=x.device, dtype=torch.float64) / rot)
+    a = (positions[axis.long()].double().t() * freq)[:, None]
+    c, s = a.cos(), a.sin()
+    u, w = (x[..., :rot // 2], x[..., rot // 2:rot]) if pairing == N.ROPE_HALF else (x[..., 0:rot:2], x[..., 1:rot:2])
+    parts, size = (u * c - w * s, w * c + u * s), u.abs() + w.abs()
+    if pairing == N.ROPE_HALF:
+        r, z = torch.cat(parts, -1), torch.cat([size, size], -1)
+    else:
+        r, z = (torch.stack(p, -1).flatten(-2) for p in (parts, (size, size)))
+    return torch.cat([r, x[..., rot:]], -1), torch.cat([z, x[..., rot:].abs()], -1)
+
+
+def rope_tolerance(dtype, want, size):
+    """Half a step of the type, and 32-bit arithmetic: norm (sum of up to 256 squares by eights and halves, root, two
+    products: 2^-24 * 16 of each term), sine and cosine, two products and a sum. With the angle in half turns rounded to 32 bits (2^-25 of up
+    to 1, times pi) and two units in the last place, sine and cosine are off by 2^-23.3 + 2^-23 < 2^-22 whatever their size, so an output is by
+    2^-22 (|u| + |w|) with u, w the pair: u cos - w sin may be far smaller than that where cosine and w are both near zero, which is
+    why `size` is |u| + |w| and not |u cos| + |w sin|. All in all below 2^-19 of it."""
+    half = torch.finfo(DTYPE[dtype][0]).eps / 2
+    return half * (1 + half) * want.abs() + 2.0 ** -19 * size + (2.0 ** -25 if dtype == "f16" else 0)
+
+
+@pytest.mark.parametrize("dim,rot,pairing", [(64, 64, 0), (64, 20, 0), (64, 16, 1), (128, 128, 0), (128, 128, 1), (128, 64, 0), (128, 6, 1), (256, 64, 0),
+                                             (256, 256, 1), (256, 250, 0), (256, 0, 0), (128, 34, 0)])
+@pytest.mark.parametrize("source,cache", [("f32", "bf16"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "f16")])
+@pytest.mark.parametrize("norm", [False, True])
+def test_rope_append(be, dim, rot, pairing, source, cache, norm):
+    heads, kv_heads, page, T, axes = 5, 3, 16, 37, 3
+    g = torch.Generator(device="cuda").manual_seed(dim + rot)
+    x = (torch.randn(T, heads + 2 * kv_heads, dim, generator=g, device="cuda") * 1.7).to(DTYPE[source][0])
+    positions = torch.randint(0, 1 << 20, (axes, T), generator=g, device="cuda", dtype=torch.int32)
+    axis = torch.randint(0, axes, (rot // 2,), generator=g, device="cuda")
+    c = Cache([90], kv_heads, dim, page, cache, layout=["nhd", "hnd", "both"][rot % 3])
+    slots = torch.randperm(c.n_pages * page, generator=g, device="cuda")[:T].int()
+    slots[3], slots[20] = -1, -100
+    wq, wk = (torch.randn(dim, generator=g, device="cuda") * 0.3 for _ in range(2))
+    q_out = torch.full((T, heads, dim), 9.0, device="cuda").to(DTYPE[cache][0])
+    k0, v0 = c.k.clone(), c.v.clone()
+    at = [x.data_ptr() + i * dim * x.element_size() for i in (0, heads, heads + kv_heads)]
+    s = x.stride()
+    op = ctox.RopeAppend(axis=axis.tolist(), tokens=T, heads=heads, kv_heads=kv_heads, dim=dim, rot_dim=rot, axes=axes, pairing=pairing,
+                         source_dtype=DTYPE[source][1], rope_base=1e6, positions=positions.data_ptr(), position_stride=T, q=at[0], k=at[1], v=at[2],
+                         q_token_stride=s[0], q_head_stride=s[1], k_token_stride=s[0], k_head_stride=s[1], v_token_stride=s[0], v_head_stride=s[1],
+                         q_norm=wq.data_ptr() if norm else None, k_norm=wk.data_ptr() if norm else None, norm_offset=1.0, norm_eps=1e-5,
+                         q_out=q_out.data_ptr(), q_out_token_stride=q_out.stride(0), q_out_head_stride=q_out.stride(1), slots=slots.data_ptr(), kv=c.op())
+    be.rope_append(op)
+    torch.cuda.synchronize()
+    assert be.device_error() == 0
+    rope = lambda h, w: rope64(h, w if norm else None, 1.0, 1e-5, positions, axis, 1e6, rot, pairing)
+    want, size = rope(x[:, :heads], wq)
+    assert near(q_out, want, rope_tolerance(cache, want, size))
+    want, size = rope(x[:, heads:heads + kv_heads], wk)
+    real = slots >= 0
+    place = slots[real].long()
+    got = c.k[place // page, place % page]
+    assert near(got, want[real], rope_tolerance(cache, want, size)[real])
+    v0[place // page, place % page] = x[real, heads + kv_heads:].to(DTYPE[cache][0])
+    k0[place // page, place % page] = got
+    bits = lambda t: t.contiguous().view(torch.int16)
+    assert torch.equal(bits(c.v), bits(v0)) and torch.equal(bits(c.k), bits(k0))  # nothing else was touched
+
+
+def test_rope_far_positions_and_halves(be):
+    """One token at a position of two thousand million: whole turns leave in 64 bits. Queries alone, keys and values alone."""
+    x = torch.randn(1, 6, 128, device="cuda")
+    positions = torch.tensor([[2 ** 31 - 1]], dtype=torch.int32, device="cuda")
+    c = Cache([20], 2, 128, 16, "f16")
+    slot = torch.tensor([5], dtype=torch.int32, device="cuda")
+    q_out = torch.zeros(1, 2, 128, device="cuda").half()
+    common = dict(tokens=1, heads=2, kv_heads=2, dim=128, rot_dim=128, axes=1, source_dtype=N.F32, rope_base=1e4, positions=positions.data_ptr(),
+                  q_token_stride=768, q_head_stride=128, k_token_stride=768, k_head_stride=128, v_token_stride=768, v_head_stride=128,
+                  q_out_token_stride=256, q_out_head_stride=128, kv=c.op(), slots=slot.data_ptr())
+    k0 = c.k.clone()
+    be.rope_append(ctox.RopeAppend(q=x.data_ptr(), q_out=q_out.data_ptr(), **common))
+    assert torch.equal(c.k.view(torch.int16), k0.view(torch.int16))
+    axis = torch.zeros(64, dtype=torch.long, device="cuda")
+    # the angle itself has an error of 2^31 * 2^-53 in the plain form too
+    want, size = rope64(x[:, :2], None, 0, 0, positions, axis, 1e4, 128, 0)
+    assert near(q_out, want, rope_tolerance("f16", want, size) + 2.0 ** -21 * size)
+    q_out.zero_()
+    be.rope_append(ctox.RopeAppend(k=x[:, 2:].data_ptr(), v=x[:, 4:].data_ptr(), **common))
+    want, size = rope64(x[:, 2:4], None, 0, 0, positions, axis, 1e4, 128, 0)
+    assert near(c.k[0, 5][None], want, rope_tolerance("f16", want, size) + 2.0 ** -21 * size)
+    assert (q_out == 0).all() and torch.equal(c.v[0, 5], x[0, 4:].half())
+
+
+def test_rope_slots_out_of_range_are_left_out(be):
+    c = Cache([20], 1, 64, 16, "bf16")
+    x = torch.randn(3, 3, 64, device="cuda")
+    slots = torch.tensor([2, c.n_pages * 16, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    q_out = torch.zeros(3, 1, 64, device="cuda").bfloat16()
+    op = ctox.RopeAppend(tokens=3, heads=1, kv_heads=1, dim=64, source_dtype=N.F32, q=x.data_ptr(), k=x[:, 1:].data_ptr(), v=x[:, 2:].data_ptr(),
+                         q_token_stride=192, q_head_stride=64, k_token_stride=192, k_head_stride=64, v_token_stride=192, v_head_stride=64,
+                         q_out=q_out.data_ptr(), q_out_token_stride=64, q_out_head_stride=64, slots=slots.data_ptr(), kv=c.op())
+    be.rope_append(op)
+    assert be.device_error() == 4
+    assert torch.equal(q_out, x[:, :1].bfloat16()) and torch.equal(c.k[0, 2], x[0, 1:2].bfloat16())
+
+
+# ---- a run of all together ----
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_server_of_requests(be, graph):
+    """Prompts, then decode steps and more prompts, over two layers; every step's attention against 64 bits over what was appended. With a
+    graph the steps are one captured program of sixteen tokens for six requests, replayed."""
+    stream = torch.cuda.Stream()
+    be = ctox.B200Backend(0, stream=stream.cuda_stream)
+    heads, kv_heads, dim, page, rot, layers, n, room = 8, 2, 128, 16, 64, 2, 6, 400
+    rng = random.Random(1)
+    m = Manager([0] * n, page, 60, 360)
+    d = m.device()
+    caches = []
+    for i in range(layers):
+        c = Cache([0] * n, kv_heads, dim, page, "bf16", seed=i)
+        c.n_pages = 360
+        c.k, c.v = (torch.full((360, page, kv_heads, dim), float("nan"), device="cuda").bfloat16() for _ in range(2))
+        c.table, c.rows = d["table"], d["rows"]
+        c.key, c.value = [torch.zeros(0, kv_heads, dim, device="cuda").bfloat16() for _ in range(n)], [torch.zeros(0, kv_heads, dim, device="cuda").bfloat16() for _ in range(n)]
+        caches.append(c)
+    if graph:
+        room = 40
+    x = [torch.zeros(room, heads + 2 * kv_heads, dim, device="cuda") for _ in range(layers)]
+    q = [torch.zeros(room, heads, dim, device="cuda").bfloat16() for _ in range(layers)]
+    out = [torch.zeros_like(t) for t in q]
+    torch.cuda.synchronize()
+    op, o = slots_op(m, d, [0] * n, room)
+    steps = []
+    for i, c in enumerate(caches):
+        s = x[i].stride()
+        at = [x[i].data_ptr() + h * dim * 4 for h in (0, heads, heads + kv_heads)]
+        rope = ctox.RopeAppend(tokens=room, heads=heads, kv_heads=kv_heads, dim=dim, rot_dim=rot, axes=1, source_dtype=N.F32, rope_base=1e4,
+                               positions=o["positions"].data_ptr(), q=at[0], k=at[1], v=at[2], q_token_stride=s[0], q_head_stride=s[1],
+                               k_token_stride=s[0], k_head_stride=s[1], v_token_stride=s[0], v_head_stride=s[1], q_out=q[i].data_ptr(),
+                               q_out_token_stride=q[i].stride(0), q_out_head_stride=q[i].stride(1), slots=o["slots"].data_ptr(), kv=c.op())
+        c.lens = [1] * n
+        att, keep = attention_op(be, c, q[i], out[i], [1] * n, max_new_tokens=room, max_kv_tokens=960,
+                                 query_offsets=o["offsets"].data_ptr(), kv_lens=o["lens_out"].data_ptr())
+        steps.append((rope, att, keep))
+
+    def step():
+        be.page_slots(op)
+        for rope, att, _ in steps:
+            be.rope_append(rope)
+            be.paged_attention(att)
+
+    if graph:
+        captured = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(captured, stream=stream):
+            step()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for t in range(12):
+        new = [rng.choice([1, 1, 1, 0, 3, rng.randint(2, 5 if graph else 60)]) for _ in range(n)]
+        if t == 0:
+            new = [5] * n if graph else [50, 3, 70, 1, 20, 100]
+        o["new"].copy_(torch.tensor(new, dtype=torch.int32))
+        for a in x:
+            a.copy_(torch.randn(a.shape, generator=g, device="cuda"))
+        for a in out:
+            a.fill_(5.0)
+        torch.cuda.synchronize()
+        captured.replay() if graph else step()
+        torch.cuda.synchronize()
+        slots, positions, requests, offsets, taken = m.take(new)
+        assert o["status"].tolist() == [taken, 0] and o["offsets"].tolist() == offsets and be.device_error() == 0
+        T = offsets[-1]
+        for i, c in enumerate(caches):
+            pos = torch.tensor([positions], dtype=torch.int32, device="cuda")
+            axis = torch.zeros(rot // 2, dtype=torch.long, device="cuda")
+            want, size = rope64(x[i][:T, heads:heads + kv_heads], None, 0, 0, pos, axis, 1e4, rot, 0)
+            place = torch.tensor(slots, device="cuda")
+            got = c.k[place // page, place % page]
+            assert near(got, want, rope_tolerance("bf16", want, size))
+            for r in range(n):
+                c.key[r] = torch.cat([c.key[r], got[offsets[r]:offsets[r + 1]]])
+                c.value[r] = torch.cat([c.value[r], x[i][offsets[r]:offsets[r + 1], heads + kv_heads:].bfloat16()])
+            c.lens = list(m.lens)
+            want, size = attention64(c, q[i][:T], new)
+            assert near(out[i][:T], want, attention_tolerance("bf16", want, size, 960))
+            assert (out[i][T:] == 5.0).all()
+    if graph:
+        del captured
+    be.close()

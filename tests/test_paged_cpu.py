@@ -1,0 +1,253 @@
+"""Operators over a paged K/V cache, what needs no GPU: refusals, struct layouts, and how attention deals its work to CTAs."""
+import ctypes as C
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+import ctox_llm_b200 as ctox
+from ctox_llm_b200 import _native as N
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+P = 0x10000  # any aligned address: nothing is read without a context
+
+
+def kv(**more):
+    return ctox.PagedKV(**{**dict(k=P, v=P, dtype=N.BF16, page_tokens=16, n_pages=100, page_stride=16 * 4 * 128, token_stride=4 * 128,
+                                  head_stride=128), **more})
+
+
+def slots_op(**more):
+    return ctox.PageSlots(**{**dict(n_requests=3, page_tokens=16, n_pages=100, table_rows=4, max_pages=10, n_tokens=50, new_tokens=P,
+                                    kv_lens_in=P, kv_lens_out=P, block_table=P, table_stride=10, free_pages=P, free_count_in=P,
+                                    free_count_out=P, query_offsets=P, slots=P, positions=P, status=P), **more})
+
+
+def release_op(**more):
+    return ctox.PageRelease(**{**dict(n_requests=3, page_tokens=16, n_pages=100, table_rows=4, max_pages=10, kv_lens=P, block_table=P,
+                                      table_stride=10, free_pages=P, free_count_in=P, free_count_out=P, status=P), **more})
+
+
+def rope_op(**more):
+    return ctox.RopeAppend(**{**dict(tokens=5, heads=8, kv_heads=4, dim=128, rot_dim=64, axes=1, pairing=N.ROPE_HALF, source_dtype=N.F32,
+                                     rope_base=1e4, positions=P, q=P, k=P, v=P, q_token_stride=1024, q_head_stride=128, k_token_stride=512,
+                                     k_head_stride=128, v_token_stride=512, v_head_stride=128, norm_eps=1e-6, q_out=P,
+                                     q_out_token_stride=1024, q_out_head_stride=128, slots=P, kv=kv()), **more})
+
+
+def attention_op(**more):
+    return ctox.PagedAttention(**{**dict(n_requests=3, n_tokens=7, max_new_tokens=5, max_kv_tokens=100, heads=8, kv_heads=4, dim=128,
+                                         causal=1, scale=0.1, query_offsets=P, kv_lens=P, block_table=P, table_rows=3, max_pages=10,
+                                         table_stride=10, q=P, q_token_stride=1024, q_head_stride=128, out=P, out_token_stride=1024,
+                                         out_head_stride=128, kv=kv()), **more})
+
+
+CALLS = {"ctox_page_slots": slots_op, "ctox_page_release": release_op, "ctox_rope_append": rope_op, "ctox_paged_attention": attention_op}
+SHAPE, DTYPE, OPERATION = "Shape", "UnsupportedDType", "UnsupportedOperation"
+REFUSED = [
+    *(("ctox_page_slots", SHAPE, f) for f in (
+        dict(n_requests=0), dict(n_requests=2049), dict(page_tokens=0), dict(page_tokens=24), dict(n_pages=0), dict(n_pages=1 << 28),
+        dict(table_rows=0), dict(max_pages=0), dict(table_stride=9), dict(max_pages=1 << 28, table_stride=1 << 28), dict(n_tokens=1 << 31),
+        dict(new_tokens=None), dict(kv_lens_in=None), dict(kv_lens_out=None), dict(block_table=None), dict(free_pages=None),
+        dict(free_count_in=None), dict(free_count_out=None), dict(query_offsets=None), dict(slots=None), dict(positions=None), dict(status=None))),
+    *(("ctox_page_release", SHAPE, f) for f in (
+        dict(n_requests=0), dict(n_requests=2049), dict(page_tokens=8), dict(table_stride=1), dict(kv_lens=None), dict(block_table=None),
+        dict(free_pages=None), dict(free_count_in=None), dict(free_count_out=None), dict(status=None))),
+    *(("ctox_rope_append", SHAPE, f) for f in (
+        dict(dim=96), dict(q=None, k=None, v=None), dict(v=None), dict(k=None), dict(heads=0), dict(kv_heads=0), dict(rot_dim=63),
+        dict(rot_dim=130), dict(positions=None), dict(axes=0), dict(axis=b"\0\1"), dict(rope_base=0.0), dict(rope_base=float("nan")),
+        dict(q_out=None), dict(q=P + 8), dict(q_token_stride=1023), dict(q_head_stride=4), dict(q_out_token_stride=4), dict(k=P + 2),
+        dict(v_head_stride=1), dict(slots=None), dict(q_norm=P + 4), dict(q_norm=P, norm_eps=-1.0), dict(k_norm=P, norm_offset=float("inf")),
+        dict(tokens=1 << 31), dict(kv=kv(k=None)), dict(kv=kv(v=P + 8)), dict(kv=kv(page_tokens=20)), dict(kv=kv(n_pages=0)),
+        dict(kv=kv(token_stride=513)), dict(kv=kv(page_stride=0)), dict(kv=kv(head_stride=0)), dict(kv=kv(page_stride=16 * 512 + 8)))),
+    ("ctox_rope_append", DTYPE, dict(source_dtype=N.Q4B64)), ("ctox_rope_append", DTYPE, dict(kv=kv(dtype=N.F32))),
+    ("ctox_rope_append", OPERATION, dict(pairing=2)),
+    *(("ctox_paged_attention", SHAPE, f) for f in (
+        dict(dim=80), dict(heads=6), dict(heads=0), dict(kv_heads=0), dict(heads=1032, kv_heads=8), dict(n_requests=0), dict(n_requests=5000),
+        dict(n_tokens=1 << 31), dict(max_new_tokens=1 << 31), dict(max_kv_tokens=1 << 31), dict(max_new_tokens=1 << 29), dict(scale=0.0),
+        dict(scale=-1.0), dict(scale=float("inf")), dict(query_offsets=None), dict(kv_lens=None), dict(block_table=None), dict(table_rows=0),
+        dict(max_pages=0), dict(table_stride=9), dict(q=None), dict(out=None), dict(q=P + 2), dict(out=P + 8), dict(q_head_stride=12),
+        dict(out_token_stride=1), dict(kv=kv(n_pages=1 << 28)), dict(kv=kv(page_stride=16 * 512 + 8)))),
+    ("ctox_paged_attention", DTYPE, dict(kv=kv(dtype=N.F32))),
+    ("ctox_paged_attention", OPERATION, dict(window=5, causal=0)), ("ctox_paged_attention", OPERATION, dict(causal=2)),
+]
+
+
+def call(name, op):
+    lib = N.load()
+    rc = getattr(lib, name)(None, op)
+    return N.ERROR_NAMES[rc], lib.ctox_last_error_message(None).decode()
+
+
+@pytest.mark.parametrize("name,kind,fields", REFUSED, ids=lambda v: str(v)[:60])
+def test_refusals_come_before_the_device(name, kind, fields):
+    got, message = call(name, CALLS[name](**fields))
+    assert got == kind and message, (got, message)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_good_operation_wants_a_context(name):
+    assert call(name, CALLS[name]()) == ("InvalidState", {"ctox_page_slots": "page slots", "ctox_page_release": "page release",
+                                                          "ctox_rope_append": "rope append",
+                                                          "ctox_paged_attention": "paged attention"}[name] + ": no context")
+    assert getattr(N.load(), name)(None, None) == 1
+
+
+def test_queries_alone_and_no_rotation_are_allowed():
+    assert call("ctox_rope_append", rope_op(k=None, v=None, slots=None, kv=ctox.PagedKV(dtype=N.F16)))[0] == "InvalidState"
+    assert call("ctox_rope_append", rope_op(q=None, q_out=None, heads=0, rot_dim=0, positions=None, axes=0))[0] == "InvalidState"
+
+
+def test_struct_layouts_match_the_header(tmp_path):
+    pairs = {"ctox_paged_kv": N.PagedKV, "ctox_page_slots_op": N.PageSlots, "ctox_page_release_op": N.PageRelease,
+             "ctox_rope_append_op": N.RopeAppend, "ctox_paged_attention_op": N.PagedAttention}
+    src = ['#include <stdio.h>', '#include <stddef.h>', '#include "ctox_b200.h"', 'int main(void){']
+    want = []
+    for name, cls in pairs.items():
+        src.append(f'printf("%zu\\n", sizeof({name}));')
+        want.append(C.sizeof(cls))
+        for f, _ in cls._fields_:
+            src.append(f'printf("%zu\\n", offsetof({name}, {f}));')
+            want.append(getattr(cls, f).offset)
+    (tmp_path / "layout.c").write_text("\n".join(src + ["return 0;}"]))
+    subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(tmp_path / "layout.c"), "-o", str(tmp_path / "layout")])
+    assert [int(x) for x in subprocess.check_output([str(tmp_path / "layout")]).split()] == want
+
+
+# ---- the dealing of attention's work (csrc/paged_plan.cuh), compiled for the host ----
+WALK = r"""
+#include "paged_plan.cuh"
+#include <vector>
+using namespace ctox::paged;
+struct HostLine {
+    const Request *q; const uint64_t *places; uint32_t n;
+    uint64_t at(uint32_t i) const { return places[i]; }
+    void request(uint32_t i, Request &r) const { r = q[i]; }
+};
+// rows out: cta, request, head, block, first tile of the unit, tile0, tile1, begins, ends, sharers (where it begins and goes on)
+extern "C" long deal(const Shape *s, const Request *q, uint32_t n, uint32_t ctas, uint32_t least, uint32_t *out, long room) {
+    std::vector<uint64_t> at(n + 1, 0);
+    for (uint32_t i = 0; i < n; ++i) {
+        uint64_t cost = 0;
+        for (uint32_t b = 0; b < blocks_of(*s, q[i]); ++b) cost += unit_of(*s, q[i], b).cost;
+        at[i + 1] = at[i] + cost * s->kv_heads;
+    }
+    const HostLine line{q, at.data(), n};
+    const uint64_t total = at[n];
+    if (!total) return 0;
+    const uint32_t pieces = pieces_of(total, ctas, least);
+    long k = 0;
+    for (uint32_t c = 0; c < pieces; ++c) {
+        Walk w;
+        w.at = cut_at(*s, line, total, pieces, c, least);
+        w.end = cut_at(*s, line, total, pieces, c + 1, least).x;
+        for (; walk_unit(*s, line, w); walk_on(*s, line, w)) {
+            if (k >= room) return -1;
+            const uint32_t r[10] = {c, w.at.request, w.at.head, w.at.block, w.u.tile0, w.tile0, w.tile1, w.begins, w.ends,
+                                    w.begins && !w.ends ? sharers(total, pieces, c, w.at.start + w.u.cost) : 0};
+            for (uint32_t j = 0; j < 10; ++j) out[k * 10 + j] = r[j];
+            ++k;
+        }
+    }
+    return k;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def deal(tmp_path_factory):
+    d = tmp_path_factory.mktemp("plan")
+    (d / "deal.cpp").write_text(WALK)
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(ROOT, "ctox_llm_b200", "csrc"), str(d / "deal.cpp"),
+                           "-o", str(d / "deal.so")])
+    lib = C.CDLL(str(d / "deal.so"))
+    lib.deal.restype = C.c_long
+
+    def run(shape, requests, ctas, least):
+        s = np.array([shape[k] for k in ("kv_heads", "group", "block_rows", "key_tile", "half_rows", "overhead", "least_rows", "most_rows",
+                                         "causal", "window")], dtype=np.uint32)
+        q = np.array(requests, dtype=np.uint32).reshape(-1, 3)
+        out = np.zeros((400000, 10), dtype=np.uint32)
+        n = lib.deal(s.ctypes.data_as(C.c_void_p), q.ctypes.data_as(C.c_void_p), len(q), ctas, least, out.ctypes.data_as(C.c_void_p), len(out))
+        assert n >= 0
+        return out[:n].astype(np.int64)
+
+    return run
+
+
+def seen(shape, new, kv, row):
+    """Keys that one row sees: (first, behind the last)."""
+    if not shape["causal"]:
+        return 0, kv
+    last = kv - new + row // shape["group"]
+    hi = min(kv, max(0, last + 1))
+    return min(hi, max(0, last + 1 - shape["window"]) if shape["window"] else 0), hi
+
+
+def draw(rng):
+    shape = dict(kv_heads=int(rng.integers(1, 9)), group=int(rng.integers(1, 9)), block_rows=int(rng.choice([8, 16, 128, 256])),
+                 key_tile=int(rng.choice([64, 128])), overhead=int(rng.integers(1, 9)), least_rows=1, most_rows=1 << 30, causal=int(rng.random() < 0.8),
+                 window=0)
+    shape["half_rows"] = 128 if shape["block_rows"] == 256 else shape["block_rows"]
+    if shape["causal"] and rng.random() < 0.4:
+        shape["window"] = int(rng.integers(1, 700))
+    if rng.random() < 0.3:
+        shape["least_rows"] = int(rng.integers(1, 40))
+    if rng.random() < 0.3:
+        shape["most_rows"] = int(rng.integers(1, 40))
+    requests = []
+    for _ in range(int(rng.integers(1, 40))):
+        new = int(rng.choice([0, 1, 1, 1, 4, rng.integers(1, 600)]))
+        kv = new + int(rng.choice([0, 3, rng.integers(0, 200), rng.integers(0, 20000)])) - int(rng.random() < 0.1) * int(rng.integers(0, 5))
+        requests.append((0, new, max(kv, 0)))
+    return shape, requests, int(rng.choice([1, 3, 148])), int(rng.integers(shape["overhead"] + 1, 20))
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_every_tile_is_dealt_once(deal, seed):
+    rng = np.random.default_rng(seed)
+    shape, requests, ctas, least = draw(rng)
+    got = deal(shape, requests, ctas, least)
+    units, slots, loads = {}, set(), {}
+    for c, r, h, b, first, t0, t1, begins, ends, share in got.tolist():
+        assert c < ctas and t0 <= t1
+        units.setdefault((r, h, b), []).append((c, first, t0, t1, begins, ends, share))
+        if not (begins and ends):  # one place per CTA for a unit that began before it, one for one that goes on
+            assert (c, begins) not in slots
+            slots.add((c, begins))
+        loads[c] = loads.get(c, 0) + (t1 - t0)
+    want = {(r, h, b) for r, (_, new, _) in enumerate(requests) for h in range(shape["kv_heads"])
+            if shape["least_rows"] <= new * shape["group"] <= shape["most_rows"]
+            for b in range(-(-new * shape["group"] // shape["block_rows"]))}
+    assert set(units) == want
+    for (r, h, b), parts in units.items():
+        _, new, kv = requests[r]
+        row0 = b * shape["block_rows"]
+        rows = range(row0, min(row0 + shape["block_rows"], new * shape["group"]))
+        ranges = [seen(shape, new, kv, x) for x in (rows[0], rows[-1])]
+        lo, hi = min(x for x, _ in ranges), max(x for _, x in ranges)
+        K = shape["key_tile"]
+        tiles = -(-hi // K) - lo // K if hi > lo else 0
+        assert all(p[1] == lo // K for p in parts)
+        assert parts[0][2] == 0 and parts[-1][3] == tiles and all(p[3] == q[2] for p, q in zip(parts, parts[1:]))
+        assert [p[0] for p in parts] == list(range(parts[0][0], parts[0][0] + len(parts)))  # neighbours, as the merge reads them
+        assert parts[0][4] and parts[-1][5] and not any(p[4] for p in parts[1:]) and not any(p[5] for p in parts[:-1])
+        if len(parts) > 1:
+            assert parts[0][6] == len(parts)
+            assert shape["overhead"] + tiles * (2 if len(rows) > shape["half_rows"] else 1) >= 2 * least
+        else:
+            assert parts[0][6] == 0
+
+
+def test_long_contexts_are_dealt_evenly(deal):
+    shape = dict(kv_heads=4, group=6, block_rows=8, key_tile=64, half_rows=8, overhead=2, least_rows=1, most_rows=16, causal=1, window=0)
+    got = deal(shape, [(0, 1, 32769)], 148, 4)
+    loads = np.bincount(got[:, 0], weights=got[:, 6] - got[:, 5])
+    assert len(loads) == 148 and loads.max() - loads.min() <= 4 and loads.sum() == 4 * 513
+
+
+def test_a_million_tokens_do_not_overflow(deal):
+    shape = dict(kv_heads=32, group=4, block_rows=8, key_tile=64, half_rows=8, overhead=2, least_rows=1, most_rows=16, causal=1, window=0)
+    got = deal(shape, [(0, 1, 1 << 24)] * 300, 148, 4)  # 2.5e9 tiles
+    assert int((got[:, 6] - got[:, 5]).sum()) == 300 * 32 * (1 << 18)
