@@ -1,4 +1,4 @@
-// Attention over a paged K/V cache for requests with few rows (a decode step, a verify pass of a few drafts), the merge of what
+// Attention over a paged K/V cache: requests with few rows (a decode step, a verify pass of a few drafts), the merge of what
 // CTAs share, and the entry points.
 //
 // With up to sixteen rows per KV head the work is the cache's bytes: about 1 flop per byte and row, so the kernel is built
@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kStages = 3;
 constexpr uint32_t kMostCtas = 160;  // one per SM
+constexpr uint32_t kFewRows = 16;    // requests with more rows are paged_attention_tile.cu's
 
 template <int D, int NT>
 struct Rows {
@@ -348,67 +349,77 @@ __global__ void __launch_bounds__(Rows<D, NT>::NW * 32 + 32)
 }
 
 // What several CTAs share. Each holds the maximum, sum and output of its keys; with M the largest maximum, weights 2^(m - M) bring
-// them to one scale, in the order of the CTAs. A block takes 1024 / D rows of one unit, four dimensions per thread; its weights once
-// in shared memory.
-constexpr uint32_t kMergeThreads = 256;
+// them to one scale, in the order of the CTAs. A block takes 1024 / D rows of one unit at a time, four dimensions per thread; its weights
+// once in shared memory. blockIdx.z: units of the kernel for few rows, of the one for many.
+constexpr uint32_t kMergeThreads = 256, kMergeBlocks = 8;
+
+struct MergePart {
+    const Shared *shared;
+    const float *partial;
+    uint32_t block_rows;
+};
 
 template <typename T>
-__global__ void __launch_bounds__(kMergeThreads) k_attention_merge(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kMergeThreads) k_attention_merge(const __grid_constant__ AttnArgs a, MergePart part0, MergePart part1) {
     __shared__ float weight[kMostCtas][16];
     __shared__ float scale[16];
-    const uint32_t D = a.op.dim, BR = a.shape.block_rows, per = 4 * kMergeThreads / D, row_first = blockIdx.y * per;
+    const MergePart p = blockIdx.z ? part1 : part0;
+    const uint32_t D = a.op.dim, BR = p.block_rows, per = 4 * kMergeThreads / D;
     pdl_launch();
     pdl_wait();
-    const Shared s = a.shared[blockIdx.x];
-    if (!s.sharers || row_first >= s.rows) return;
+    const Shared s = p.shared[blockIdx.x];
+    if (!s.sharers) return;
     const uint64_t slot = slot_floats(BR, D);
-    auto slot_of = [&](uint32_t i) { return a.partial + ((uint64_t)(blockIdx.x + i) * 2 + (i ? 0 : 1)) * slot; };
+    auto slot_of = [&](uint32_t i) { return p.partial + ((uint64_t)(blockIdx.x + i) * 2 + (i ? 0 : 1)) * slot; };
     Request q;
     read_request(a, s.request, q);
     const uint32_t tid = threadIdx.x, group = a.shape.group;
-    for (uint32_t i = tid; i < s.sharers * per; i += kMergeThreads)
-        if (row_first + i % per < s.rows) weight[i / per][i % per] = slot_of(i / per)[row_first + i % per];
-    __syncthreads();
-    if (tid < per && row_first + tid < s.rows) {
-        float top = -INFINITY;
-        for (uint32_t i = 0; i < s.sharers; ++i) top = fmaxf(top, weight[i][tid]);
-        float sum = 0.f;
-        for (uint32_t i = 0; i < s.sharers; ++i) {
-            const float l = slot_of(i)[BR + row_first + tid];
-            // a part that saw nothing for this row has sum 0
-            const float f = l == 0.f ? 0.f : umma::ex2(weight[i][tid] - top);
-            weight[i][tid] = f;
-            if (l != 0.f) sum += f * l;
+    for (uint32_t row_first = blockIdx.y * per; row_first < s.rows; row_first += gridDim.y * per) {
+        const uint32_t rows = min(per, s.rows - row_first);
+        __syncthreads();
+        for (uint32_t i = tid; i < s.sharers * per; i += kMergeThreads)
+            if (i % per < rows) weight[i / per][i % per] = slot_of(i / per)[row_first + i % per];
+        __syncthreads();
+        if (tid < rows) {
+            float top = -INFINITY;
+            for (uint32_t i = 0; i < s.sharers; ++i) top = fmaxf(top, weight[i][tid]);
+            float sum = 0.f;
+            for (uint32_t i = 0; i < s.sharers; ++i) {
+                const float l = slot_of(i)[BR + row_first + tid];
+                // a part that saw nothing for this row has sum 0
+                const float f = l == 0.f ? 0.f : umma::ex2(weight[i][tid] - top);
+                weight[i][tid] = f;
+                if (l != 0.f) sum += f * l;
+            }
+            const uint32_t r = s.row0 + row_first + tid;
+            if (sum != 0.f && a.op.sinks) sum += umma::ex2(fmaf(a.op.sinks[s.head * group + r % group], 1.4426950408889634f, -top));
+            scale[tid] = sum == 0.f ? 0.f : 1.0f / sum;
         }
-        const uint32_t r = s.row0 + row_first + tid;
-        if (sum != 0.f && a.op.sinks)
-            sum += umma::ex2(fmaf(a.op.sinks[s.head * group + r % group], 1.4426950408889634f, -top));
-        scale[tid] = sum == 0.f ? 0.f : 1.0f / sum;
-    }
-    __syncthreads();
-    const uint32_t in = tid % per, d4 = tid / per, row = row_first + in;
-    if (row >= s.rows) return;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        __syncthreads();
+        const uint32_t in = tid % per, d4 = tid / per, row = row_first + in;
+        if (in >= rows) continue;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-    for (uint32_t i = 0; i < s.sharers; ++i) {
-        const float f = weight[i][in];
-        const float4 x = reinterpret_cast<const float4 *>(slot_of(i) + 2 * BR)[d4 * BR + row];
-        if (f != 0.f) {
-            o.x = fmaf(f, x.x, o.x);
-            o.y = fmaf(f, x.y, o.y);
-            o.z = fmaf(f, x.z, o.z);
-            o.w = fmaf(f, x.w, o.w);
+        for (uint32_t i = 0; i < s.sharers; ++i) {
+            const float f = weight[i][in];
+            const float4 x = reinterpret_cast<const float4 *>(slot_of(i) + 2 * BR)[d4 * BR + row];
+            if (f != 0.f) {
+                o.x = fmaf(f, x.x, o.x);
+                o.y = fmaf(f, x.y, o.y);
+                o.z = fmaf(f, x.z, o.z);
+                o.w = fmaf(f, x.w, o.w);
+            }
         }
+        const uint32_t r = s.row0 + row;
+        const float f = scale[in];
+        T *out = (T *)a.op.out + (uint64_t)(q.q0 + r / group) * a.op.out_token_stride +
+                 (uint64_t)(s.head * group + r % group) * a.op.out_head_stride + d4 * 4;
+        *reinterpret_cast<uint2 *>(out) = make_uint2(pack_pair<T>(o.x * f, o.y * f), pack_pair<T>(o.z * f, o.w * f));
     }
-    const uint32_t r = s.row0 + row;
-    const float f = scale[in];
-    T *out = (T *)a.op.out + (uint64_t)(q.q0 + r / group) * a.op.out_token_stride +
-             (uint64_t)(s.head * group + r % group) * a.op.out_head_stride + d4 * 4;
-    *reinterpret_cast<uint2 *>(out) = make_uint2(pack_pair<T>(o.x * f, o.y * f), pack_pair<T>(o.z * f, o.w * f));
 }
 
 template <typename T, int D, int NT>
-ctox_status rows_launch(ctox_ctx *ctx, AttnArgs a) {
+ctox_status rows_launch(ctox_ctx *ctx, AttnArgs &a) {
     using R = Rows<D, NT>;
     a.shape.block_rows = R::BR;
     a.shape.half_rows = R::BR;
@@ -421,22 +432,15 @@ ctox_status rows_launch(ctox_ctx *ctx, AttnArgs a) {
     const size_t smem = R::smem(a.op.n_requests);
     auto kernel = k_attention_rows<T, D, NT>;
     CTOX_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const uint32_t grid = (uint32_t)ctx->sm_count;
-    CTOX_CUDA(ctx, launch_pdl(kernel, dim3(grid), dim3(R::NW * 32 + 32), smem, ctx->stream, mk, mv, a, ctx->dev_error));
-    // the longest unit that there can be: where not even that is cut, there is nothing to merge
-    const uint32_t most = a.shape.overhead + (a.op.max_kv_tokens + R::KT - 1) / R::KT;
-    if (keeps_whole(most, a.least)) return CTOX_OK;
-    const uint32_t per = 4 * kMergeThreads / D;
-    CTOX_CUDA(ctx, launch_pdl(k_attention_merge<T>, dim3(grid, (R::BR + per - 1) / per), dim3(kMergeThreads), 0, ctx->stream, a));
+    CTOX_CUDA(ctx, launch_pdl(kernel, dim3((uint32_t)ctx->sm_count), dim3(R::NW * 32 + 32), smem, ctx->stream, mk, mv, a, ctx->dev_error));
     return CTOX_OK;
 }
 template <typename T, int D>
-ctox_status rows_launch(ctox_ctx *ctx, const AttnArgs &a) {
-    const uint64_t rows = (uint64_t)a.op.max_new_tokens * a.shape.group;
-    return rows <= 8 ? rows_launch<T, D, 1>(ctx, a) : rows_launch<T, D, 2>(ctx, a);
+ctox_status rows_launch(ctox_ctx *ctx, AttnArgs &a) {
+    return a.shape.most_rows <= 8 ? rows_launch<T, D, 1>(ctx, a) : rows_launch<T, D, 2>(ctx, a);
 }
 template <typename T>
-ctox_status rows_launch(ctox_ctx *ctx, const AttnArgs &a) {
+ctox_status rows_launch(ctox_ctx *ctx, AttnArgs &a) {
     return a.op.dim == 64 ? rows_launch<T, 64>(ctx, a) : a.op.dim == 128 ? rows_launch<T, 128>(ctx, a) : rows_launch<T, 256>(ctx, a);
 }
 
@@ -470,7 +474,7 @@ ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attentio
     return CTOX_OK;
 }
 
-ctox_status launch_attention_rows(ctox_ctx *ctx, const AttnArgs &a) {
+ctox_status launch_attention_rows(ctox_ctx *ctx, AttnArgs &a) {
     return a.op.kv.dtype == CTOX_BF16 ? rows_launch<__nv_bfloat16>(ctx, a) : rows_launch<__half>(ctx, a);
 }
 
@@ -482,8 +486,11 @@ static ctox_status check_heads(ctox_ctx *ctx, const ctox_paged_attention_op *op)
         return fail(ctx, CTOX_SHAPE, "%s: %u query heads over %u KV heads (a multiple, up to 128 times)", what, op->heads, op->kv_heads);
     return CTOX_OK;
 }
+// Two descriptors per CTA, two slots of few rows, two of many.
+static uint64_t descriptor_bytes(const ctox_ctx *ctx) { return (2 * ctx->sm_count * sizeof(Shared) + 255) & ~255ull; }
+static uint64_t rows_floats(const ctox_ctx *ctx, uint32_t dim) { return (uint64_t)ctx->sm_count * 2 * slot_floats(kFewRows, dim); }
 static uint64_t workspace_bytes(const ctox_ctx *ctx, const ctox_paged_attention_op &op) {
-    return (uint64_t)ctx->sm_count * (2 * slot_floats(16, op.dim) * 4 + sizeof(Shared)) + 256;
+    return descriptor_bytes(ctx) + rows_floats(ctx, op.dim) * 4 + (uint64_t)ctx->sm_count * 2 * slot_floats(tile_block_rows(op.dim), op.dim) * 4;
 }
 
 }  // namespace paged
@@ -534,17 +541,46 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
     a.shape.group = op->heads / op->kv_heads;
     a.shape.causal = op->causal;
     a.shape.window = op->window;
-    a.shape.least_rows = 1;
-    a.shape.most_rows = 0x7fffffffu;
-    a.shape.overhead = 2;
-    a.least = 4;
     a.pages_per_step = op->kv_heads > 1 ? (uint32_t)(op->kv.page_stride / op->kv.head_stride) : 1;
     a.c = op->scale * 1.4426950408889634f;
-    a.shared = (Shared *)op->workspace;
-    a.partial = (float *)((uint8_t *)op->workspace + ((ctx->sm_count * sizeof(Shared) + 255) & ~255ull));
     const DeviceGuard guard(ctx->device);
     CTOX_CUDA(ctx, guard.error());
-    return launch_attention_rows(ctx, a);
+    // Only the device knows how many rows a request has; the host knows the most, and that a token has `group`.
+    const uint64_t most = (uint64_t)op->max_new_tokens * a.shape.group;
+    const bool many = most > kFewRows, few = !many || (op->n_requests > 1 && a.shape.group <= kFewRows);
+    MergePart parts[2] = {};
+    uint32_t n_parts = 0;
+    auto merged = [&](uint32_t tile_cost) {  // where not even the longest unit that there can be is cut, there is nothing to merge
+        const uint64_t longest = a.shape.overhead + ((uint64_t)op->max_kv_tokens + a.shape.key_tile - 1) / a.shape.key_tile * tile_cost;
+        if (longest <= 0xffffffffu && keeps_whole((uint32_t)longest, a.least)) return;
+        parts[n_parts++] = MergePart{a.shared, a.partial, a.shape.block_rows};
+    };
+    if (few) {
+        a.shape.least_rows = 1;
+        a.shape.most_rows = many ? kFewRows : (uint32_t)most;
+        a.shape.overhead = 2;
+        a.least = 4;
+        a.shared = (Shared *)op->workspace;
+        a.partial = (float *)((uint8_t *)op->workspace + descriptor_bytes(ctx));
+        EX(launch_attention_rows(ctx, a));
+        merged(1);
+    }
+    if (many) {
+        a.shape.least_rows = few ? kFewRows + 1 : 1;
+        a.shape.most_rows = (uint32_t)most;
+        a.shape.overhead = 3;
+        a.least = 6;
+        a.shared = (Shared *)op->workspace + ctx->sm_count;
+        a.partial = (float *)((uint8_t *)op->workspace + descriptor_bytes(ctx)) + rows_floats(ctx, op->dim);
+        EX(launch_attention_tile(ctx, a));
+        merged(2);
+    }
+    if (n_parts) {
+        const dim3 grid((uint32_t)ctx->sm_count, kMergeBlocks, n_parts);
+        CTOX_CUDA(ctx, op->kv.dtype == CTOX_BF16 ? launch_pdl(k_attention_merge<__nv_bfloat16>, grid, dim3(kMergeThreads), 0, ctx->stream, a, parts[0], parts[1])
+                                                 : launch_pdl(k_attention_merge<__half>, grid, dim3(kMergeThreads), 0, ctx->stream, a, parts[0], parts[1]));
+    }
+    return CTOX_OK;
 }
 
 }  // extern "C"

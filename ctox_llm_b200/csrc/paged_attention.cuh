@@ -98,7 +98,9 @@ __device__ __forceinline__ int box_step(const AttnArgs &a, int32_t page, uint32_
 ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attention_op &op, const void *base, uint32_t box, uint32_t chunks);
 
 // Requests with few rows (paged_attention.cu) and with many (paged_attention_tile.cu).
-ctox_status launch_attention_rows(ctox_ctx *ctx, const AttnArgs &a);
+ctox_status launch_attention_rows(ctox_ctx *ctx, AttnArgs &a);
+ctox_status launch_attention_tile(ctox_ctx *ctx, AttnArgs &a);
+uint32_t tile_block_rows(uint32_t dim);
 
 }  // namespace paged
 }  // namespace ctox
