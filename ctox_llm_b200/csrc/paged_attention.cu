@@ -93,15 +93,15 @@ __global__ void __launch_bounds__(Rows<D, NT>::NW * 32 + 32)
     __syncthreads();
     pdl_launch();
     pdl_wait();
-    const uint64_t total = lay_line(a, at, scan, error_word);
-    const uint32_t pieces = total ? pieces_of(total, gridDim.x, a.least) : 0;
+    lay_line(a, at, scan, reinterpret_cast<uint32_t *>(aligned), error_word);
     const Line line{a, at, a.op.n_requests};
-    if (blockIdx.x >= pieces) {
+    const Cuts cut = cuts_of(at[a.op.n_requests], gridDim.x, a.least);
+    if (blockIdx.x >= cut.pieces) {
         if (tid == 0) a.shared[blockIdx.x].sharers = 0;
         return;
     }
     if (warp < 2) {
-        const Cut c = cut_at(a.shape, line, total, pieces, blockIdx.x + warp, a.least);
+        const Cut c = cut_at(a.shape, line, cut, blockIdx.x + warp);
         if (lane == 0) cuts[warp] = c;
     }
     __syncthreads();
@@ -114,18 +114,21 @@ __global__ void __launch_bounds__(Rows<D, NT>::NW * 32 + 32)
         uint32_t n = 0;
         for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
             const int32_t *table = table_row(a, w.at.request);
+            auto wanted = [&](uint32_t token) { return lane < per && token < w.u.hi && token + a.box > w.u.lo; };
+            const uint32_t first = (w.u.tile0 + w.tile0) * R::KT + lane * a.box;
+            int32_t next = w.tile0 < w.tile1 && wanted(first) ? table[page_index(a, first)] : 0;
             for (uint32_t t = w.tile0; t < w.tile1; ++t, ++n) {
                 const uint32_t s = n % kStages, round = n / kStages;
                 const uint32_t token = (w.u.tile0 + t) * R::KT + lane * a.box;
-                int32_t page = -1;
-                bool mine = lane < per && token < w.u.hi && token + a.box > w.u.lo;
-                if (mine) mine = page_at(a, table, token, page, error_word);
+                const int32_t page = next;
+                const bool mine = wanted(token) && is_page(a, page, error_word);
+                if (t + 1 < w.tile1 && wanted(token + R::KT)) next = table[page_index(a, token + R::KT)];  // on its way while this one waits
                 const uint32_t copies = __popc(__ballot_sync(0xffffffffu, mine));
                 if (round > 0 && !(ok = __all_sync(0xffffffffu, bar_wait(empty + s * 8, (round - 1) & 1, &dead)))) break;
                 if (lane == 0) bar_expect(full + s * 8, copies * 2 * box_bytes);
                 __syncwarp();
                 if (mine) {
-                    const int group = (int)(token % a.op.kv.page_tokens / 8), step = box_step(a, page, w.at.head);
+                    const int group = (int)((token - (uint32_t)page_index(a, token) * a.op.kv.page_tokens) / 8), step = box_step(a, page, w.at.head);
                     const uint32_t dst = base + s * 2 * R::TILE + lane * box_bytes;
                     load_box(dst, &map_k, full + s * 8, 0, group, step);
                     load_box(dst + R::TILE, &map_v, full + s * 8, 0, group, step);
@@ -340,7 +343,7 @@ __global__ void __launch_bounds__(Rows<D, NT>::NW * 32 + 32)
             if (w.begins) {
                 shares = true;
                 if (tid == 0)
-                    a.shared[blockIdx.x] = Shared{sharers(total, pieces, blockIdx.x, w.at.start + w.u.cost), w.at.request, w.at.head, w.u.row0, w.u.rows};
+                    a.shared[blockIdx.x] = Shared{sharers(cut, blockIdx.x, w.at.start + w.u.cost), w.at.request, w.at.head, w.u.row0, w.u.rows};
             }
         }
     }
@@ -349,73 +352,66 @@ __global__ void __launch_bounds__(Rows<D, NT>::NW * 32 + 32)
 }
 
 // What several CTAs share. Each holds the maximum, sum and output of its keys; with M the largest maximum, weights 2^(m - M) bring
-// them to one scale, in the order of the CTAs. A block takes 1024 / D rows of one unit at a time, four dimensions per thread; its weights
-// once in shared memory. blockIdx.z: units of the kernel for few rows, of the one for many.
-constexpr uint32_t kMergeThreads = 256, kMergeBlocks = 8;
+// them to one scale, in the order of the CTAs. A block takes 1024 / D rows of one unit, four dimensions per thread. The parts: units of the kernel for few rows, of the one for many.
+constexpr uint32_t kMergeThreads = 256;
 
 struct MergePart {
     const Shared *shared;
     const float *partial;
-    uint32_t block_rows;
+    uint32_t block_rows, pieces;
 };
 
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) k_attention_merge(const __grid_constant__ AttnArgs a, MergePart part0, MergePart part1) {
-    __shared__ float weight[kMostCtas][16];
-    __shared__ float scale[16];
-    const MergePart p = blockIdx.z ? part1 : part0;
-    const uint32_t D = a.op.dim, BR = p.block_rows, per = 4 * kMergeThreads / D;
+    __shared__ float top[kMostCtas][16], sum[kMostCtas][16];
+    const uint32_t D = a.op.dim, per = 4 * kMergeThreads / D;
+    // blocks of the first part, then of the second: for each piece as many as its rows want
+    const uint32_t slices0 = (part0.block_rows + per - 1) / per, blocks0 = part0.pieces * slices0;
+    const bool second = blockIdx.x >= blocks0;
+    const MergePart p = second ? part1 : part0;
+    const uint32_t BR = p.block_rows, slices = second ? (BR + per - 1) / per : slices0, block = second ? blockIdx.x - blocks0 : blockIdx.x;
+    const uint32_t piece = block / slices, row_first = block % slices * per;
     pdl_launch();
     pdl_wait();
-    const Shared s = p.shared[blockIdx.x];
-    if (!s.sharers) return;
+    const Shared s = p.shared[piece];
+    if (!s.sharers || row_first >= s.rows) return;
     const uint64_t slot = slot_floats(BR, D);
-    auto slot_of = [&](uint32_t i) { return p.partial + ((uint64_t)(blockIdx.x + i) * 2 + (i ? 0 : 1)) * slot; };
+    auto slot_of = [&](uint32_t i) { return p.partial + ((uint64_t)(piece + i) * 2 + (i ? 0 : 1)) * slot; };
     Request q;
     read_request(a, s.request, q);
     const uint32_t tid = threadIdx.x, group = a.shape.group;
-    for (uint32_t row_first = blockIdx.y * per; row_first < s.rows; row_first += gridDim.y * per) {
-        const uint32_t rows = min(per, s.rows - row_first);
-        __syncthreads();
-        for (uint32_t i = tid; i < s.sharers * per; i += kMergeThreads)
-            if (i % per < rows) weight[i / per][i % per] = slot_of(i / per)[row_first + i % per];
-        __syncthreads();
-        if (tid < rows) {
-            float top = -INFINITY;
-            for (uint32_t i = 0; i < s.sharers; ++i) top = fmaxf(top, weight[i][tid]);
-            float sum = 0.f;
-            for (uint32_t i = 0; i < s.sharers; ++i) {
-                const float l = slot_of(i)[BR + row_first + tid];
-                // a part that saw nothing for this row has sum 0
-                const float f = l == 0.f ? 0.f : umma::ex2(weight[i][tid] - top);
-                weight[i][tid] = f;
-                if (l != 0.f) sum += f * l;
-            }
-            const uint32_t r = s.row0 + row_first + tid;
-            if (sum != 0.f && a.op.sinks) sum += umma::ex2(fmaf(a.op.sinks[s.head * group + r % group], 1.4426950408889634f, -top));
-            scale[tid] = sum == 0.f ? 0.f : 1.0f / sum;
+    for (uint32_t i = tid; i < s.sharers * per; i += kMergeThreads)
+        if (row_first + i % per < s.rows) {
+            const float *x = slot_of(i / per) + row_first + i % per;
+            top[i / per][i % per] = x[0];
+            sum[i / per][i % per] = x[BR];
         }
-        __syncthreads();
-        const uint32_t in = tid % per, d4 = tid / per, row = row_first + in;
-        if (in >= rows) continue;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    __syncthreads();
+    const uint32_t in = tid % per, d4 = tid / per, row = row_first + in;
+    if (row >= s.rows) return;
+    // a part that saw nothing for this row has maximum -inf and sum 0
+    float most = -INFINITY;
+    for (uint32_t i = 0; i < s.sharers; ++i) most = fmaxf(most, top[i][in]);
+    const float ref = most == -INFINITY ? 0.f : most;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float all = 0.f;
 #pragma unroll 8
-        for (uint32_t i = 0; i < s.sharers; ++i) {
-            const float f = weight[i][in];
-            const float4 x = reinterpret_cast<const float4 *>(slot_of(i) + 2 * BR)[d4 * BR + row];
-            if (f != 0.f) {
-                o.x = fmaf(f, x.x, o.x);
-                o.y = fmaf(f, x.y, o.y);
-                o.z = fmaf(f, x.z, o.z);
-                o.w = fmaf(f, x.w, o.w);
-            }
+    for (uint32_t i = 0; i < s.sharers; ++i) {
+        const float4 x = reinterpret_cast<const float4 *>(slot_of(i) + 2 * BR)[d4 * BR + row];
+        const float f = umma::ex2(top[i][in] - ref);
+        all = fmaf(f, sum[i][in], all);
+        if (f != 0.f) {
+            o.x = fmaf(f, x.x, o.x);
+            o.y = fmaf(f, x.y, o.y);
+            o.z = fmaf(f, x.z, o.z);
+            o.w = fmaf(f, x.w, o.w);
         }
-        const uint32_t r = s.row0 + row;
-        const float f = scale[in];
-        T *out = (T *)a.op.out + (uint64_t)(q.q0 + r / group) * a.op.out_token_stride +
-                 (uint64_t)(s.head * group + r % group) * a.op.out_head_stride + d4 * 4;
-        *reinterpret_cast<uint2 *>(out) = make_uint2(pack_pair<T>(o.x * f, o.y * f), pack_pair<T>(o.z * f, o.w * f));
     }
+    const uint32_t r = s.row0 + row, head = s.head * group + r % group;
+    if (all != 0.f && a.op.sinks) all += umma::ex2(fmaf(a.op.sinks[head], 1.4426950408889634f, -ref));
+    const float f = all == 0.f ? 0.f : 1.0f / all;
+    T *out = (T *)a.op.out + (uint64_t)(q.q0 + r / group) * a.op.out_token_stride + (uint64_t)head * a.op.out_head_stride + d4 * 4;
+    *reinterpret_cast<uint2 *>(out) = make_uint2(pack_pair<T>(o.x * f, o.y * f), pack_pair<T>(o.z * f, o.w * f));
 }
 
 template <typename T, int D, int NT>
@@ -423,7 +419,7 @@ ctox_status rows_launch(ctox_ctx *ctx, AttnArgs &a) {
     using R = Rows<D, NT>;
     a.shape.block_rows = R::BR;
     a.shape.half_rows = R::BR;
-    a.shape.key_tile = R::KT;
+    a.shape.key_shift = R::KT == 64 ? 6 : 7;
     a.box = R::KT;
     while (a.op.kv.page_tokens % a.box) a.box /= 2;
     CUtensorMap mk, mv;
@@ -446,7 +442,8 @@ ctox_status rows_launch(ctox_ctx *ctx, AttnArgs &a) {
 
 }  // namespace
 
-ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attention_op &op, const void *base, uint32_t box, uint32_t chunks) {
+ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attention_op &op, const void *base, uint32_t box, uint32_t chunks,
+                      uint32_t width) {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -462,12 +459,13 @@ ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attentio
     const ctox_paged_kv &kv = op.kv;
     // one axis runs over pages and heads
     const uint64_t step = op.kv_heads > 1 ? kv.head_stride : kv.page_stride, per_page = op.kv_heads > 1 ? kv.page_stride / kv.head_stride : 1;
-    const cuuint64_t dims[5] = {64, 8, op.dim / 64, kv.page_tokens / 8, (uint64_t)(kv.n_pages - 1) * per_page + op.kv_heads};
-    const cuuint64_t strides[4] = {kv.token_stride * 2, 128, kv.token_stride * 16, step * 2};
-    const cuuint32_t boxes[5] = {64, 8, chunks, box / 8, 1}, each[5] = {1, 1, 1, 1, 1};
+    const cuuint64_t dims[5] = {width, 8, op.dim / width, kv.page_tokens / 8, (uint64_t)(kv.n_pages - 1) * per_page + op.kv_heads};
+    const cuuint64_t strides[4] = {kv.token_stride * 2, width * 2, kv.token_stride * 16, step * 2};
+    const cuuint32_t boxes[5] = {width, 8, chunks, box / 8, 1}, each[5] = {1, 1, 1, 1, 1};
     const CUresult r = encode(map, kv.dtype == CTOX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                               const_cast<void *>(base), dims, strides, boxes, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                              width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return fail(ctx, CTOX_SHAPE, "paged attention: a cache of %u pages with strides %llu, %llu, %llu has no tensor map (error %d)", kv.n_pages,
                     (unsigned long long)kv.page_stride, (unsigned long long)kv.token_stride, (unsigned long long)kv.head_stride, (int)r);
@@ -490,7 +488,7 @@ static ctox_status check_heads(ctox_ctx *ctx, const ctox_paged_attention_op *op)
 static uint64_t descriptor_bytes(const ctox_ctx *ctx) { return (2 * ctx->sm_count * sizeof(Shared) + 255) & ~255ull; }
 static uint64_t rows_floats(const ctox_ctx *ctx, uint32_t dim) { return (uint64_t)ctx->sm_count * 2 * slot_floats(kFewRows, dim); }
 static uint64_t workspace_bytes(const ctox_ctx *ctx, const ctox_paged_attention_op &op) {
-    return descriptor_bytes(ctx) + rows_floats(ctx, op.dim) * 4 + (uint64_t)ctx->sm_count * 2 * slot_floats(tile_block_rows(op.dim), op.dim) * 4;
+    return descriptor_bytes(ctx) + rows_floats(ctx, op.dim) * 4 + (uint64_t)(ctx->sm_count / 2) * 2 * slot_floats(kTileBlockRows, op.dim) * 4;
 }
 
 }  // namespace paged
@@ -543,6 +541,10 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
     a.shape.window = op->window;
     a.pages_per_step = op->kv_heads > 1 ? (uint32_t)(op->kv.page_stride / op->kv.head_stride) : 1;
     a.c = op->scale * 1.4426950408889634f;
+    uint32_t bits = 0;
+    while ((1ull << bits) < op->kv.page_tokens) ++bits;
+    a.page_shift = 31 + bits;
+    a.page_factor = (uint32_t)((1ull << a.page_shift) / op->kv.page_tokens + 1);
     const DeviceGuard guard(ctx->device);
     CTOX_CUDA(ctx, guard.error());
     // Only the device knows how many rows a request has; the host knows the most, and that a token has `group`.
@@ -550,10 +552,10 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
     const bool many = most > kFewRows, few = !many || (op->n_requests > 1 && a.shape.group <= kFewRows);
     MergePart parts[2] = {};
     uint32_t n_parts = 0;
-    auto merged = [&](uint32_t tile_cost) {  // where not even the longest unit that there can be is cut, there is nothing to merge
-        const uint64_t longest = a.shape.overhead + ((uint64_t)op->max_kv_tokens + a.shape.key_tile - 1) / a.shape.key_tile * tile_cost;
+    auto merged = [&](uint32_t ctas) {  // where not even the longest unit that there can be is cut, there is nothing to merge
+        const uint64_t longest = a.shape.overhead + ((((uint64_t)op->max_kv_tokens - 1) >> a.shape.key_shift) + 1);
         if (longest <= 0xffffffffu && keeps_whole((uint32_t)longest, a.least)) return;
-        parts[n_parts++] = MergePart{a.shared, a.partial, a.shape.block_rows};
+        parts[n_parts++] = MergePart{a.shared, a.partial, a.shape.block_rows, ctas};
     };
     if (few) {
         a.shape.least_rows = 1;
@@ -563,22 +565,24 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
         a.shared = (Shared *)op->workspace;
         a.partial = (float *)((uint8_t *)op->workspace + descriptor_bytes(ctx));
         EX(launch_attention_rows(ctx, a));
-        merged(1);
+        merged((uint32_t)ctx->sm_count);
     }
     if (many) {
         a.shape.least_rows = few ? kFewRows + 1 : 1;
         a.shape.most_rows = (uint32_t)most;
-        a.shape.overhead = 3;
-        a.least = 6;
+        a.shape.overhead = 4;
+        a.least = 8;
         a.shared = (Shared *)op->workspace + ctx->sm_count;
         a.partial = (float *)((uint8_t *)op->workspace + descriptor_bytes(ctx)) + rows_floats(ctx, op->dim);
         EX(launch_attention_tile(ctx, a));
-        merged(2);
+        merged((uint32_t)ctx->sm_count / 2);
     }
     if (n_parts) {
-        const dim3 grid((uint32_t)ctx->sm_count, kMergeBlocks, n_parts);
-        CTOX_CUDA(ctx, op->kv.dtype == CTOX_BF16 ? launch_pdl(k_attention_merge<__nv_bfloat16>, grid, dim3(kMergeThreads), 0, ctx->stream, a, parts[0], parts[1])
-                                                 : launch_pdl(k_attention_merge<__half>, grid, dim3(kMergeThreads), 0, ctx->stream, a, parts[0], parts[1]));
+        const uint32_t per = 4 * kMergeThreads / op->dim;
+        uint32_t grid = 0;
+        for (const MergePart &p : parts) grid += p.pieces * ((p.block_rows + per - 1) / per);
+        CTOX_CUDA(ctx, op->kv.dtype == CTOX_BF16 ? launch_pdl(k_attention_merge<__nv_bfloat16>, dim3(grid), dim3(kMergeThreads), 0, ctx->stream, a, parts[0], parts[1])
+                                                 : launch_pdl(k_attention_merge<__half>, dim3(grid), dim3(kMergeThreads), 0, ctx->stream, a, parts[0], parts[1]));
     }
     return CTOX_OK;
 }

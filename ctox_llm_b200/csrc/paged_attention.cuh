@@ -18,6 +18,7 @@ struct AttnArgs {
     Shape shape;
     uint32_t least;          // cost below which a piece of the work is not worth a CTA
     uint32_t box;            // tokens of a copy: what a page and a key tile are both multiples of
+    uint32_t page_factor, page_shift;  // token / page_tokens = token * page_factor >> page_shift, for tokens below 2^31
     uint32_t pages_per_step; // page_stride / head_stride where there are several heads, else 1
     float c;                 // scale * log2(e)
     float *partial;          // per CTA two slots: a unit that began before it, one that goes on behind it
@@ -42,27 +43,44 @@ __device__ __forceinline__ const int32_t *table_row(const AttnArgs &a, uint32_t 
     return a.op.block_table + (uint64_t)(a.op.rows ? a.op.rows[i] : (int32_t)i) * a.op.table_stride;
 }
 
-// Line places of all requests: at[0 .. n], by the whole block. Returns the line's length.
-__device__ __forceinline__ uint64_t lay_line(const AttnArgs &a, unsigned long long *at, unsigned long long *scan, int32_t *error_word) {
+// Line places of all requests: at[0 .. n], by the whole block (`scan`: a word per warp). A request's blocks are summed by its thread,
+// but a long prompt's thousands by all threads: such requests are put down in `list` (n words, free to use until the return).
+constexpr uint32_t kFewBlocks = 4;
+__device__ __forceinline__ void lay_line(const AttnArgs &a, unsigned long long *at, unsigned long long *scan, uint32_t *list, int32_t *error_word) {
+    __shared__ uint32_t listed;
     const uint32_t n = a.op.n_requests, per = (n + blockDim.x - 1) / blockDim.x, r0 = threadIdx.x * per;
-    unsigned long long mine = 0;
+    if (threadIdx.x == 0) listed = 0;
+    __syncthreads();
     for (uint32_t r = r0; r < r0 + per && r < n; ++r) {
         Request q;
         unsigned long long cost = 0;
         if (read_request(a, r, q)) {
             const uint32_t blocks = blocks_of(a.shape, q);
-            for (uint32_t b = 0; b < blocks; ++b) cost += unit_of(a.shape, q, b).cost;
+            if (blocks <= kFewBlocks)
+                for (uint32_t b = 0; b < blocks; ++b) cost += unit_of(a.shape, q, b).cost;
+            else
+                list[atomicAdd(&listed, 1)] = r;
         } else if (blockIdx.x == 0) {
             bad_index(error_word);
         }
-        at[r + 1] = cost * a.shape.kv_heads;
-        mine += at[r + 1];
+        at[r + 1] = cost;
     }
+    __syncthreads();
+    for (uint32_t i = 0, m = listed; i < m; ++i) {
+        Request q;
+        read_request(a, list[i], q);
+        const uint32_t blocks = blocks_of(a.shape, q);
+        unsigned long long cost = 0;
+        for (uint32_t b = threadIdx.x; b < blocks; b += blockDim.x) cost += unit_of(a.shape, q, b).cost;
+        if (cost) atomicAdd(&at[list[i] + 1], cost);
+    }
+    __syncthreads();
+    unsigned long long mine = 0;
+    for (uint32_t r = r0; r < r0 + per && r < n; ++r) mine += at[r + 1] *= a.shape.kv_heads;
     unsigned long long before = block_scan<unsigned long long>(mine, scan) - mine;
     for (uint32_t r = r0; r < r0 + per && r < n; ++r) at[r + 1] = before += at[r + 1];
     if (threadIdx.x == 0) at[0] = 0;
     __syncthreads();
-    return at[n];
 }
 
 // The line for the walks of paged_plan.cuh.
@@ -71,12 +89,19 @@ struct Line {
     const unsigned long long *places;
     uint32_t n;
     __device__ __forceinline__ uint64_t at(uint32_t i) const { return places[i]; }
+    __device__ __forceinline__ uint64_t per_head(uint32_t i) const {
+        const uint64_t all = places[i + 1] - places[i];
+        return all >> 32 ? all / a.shape.kv_heads : (uint32_t)all / a.shape.kv_heads;
+    }
     __device__ __forceinline__ void request(uint32_t i, Request &q) const { read_request(a, i, q); }
 };
 
-// Page of a token for the copies; false (and the device error) where the table's entry is none.
-__device__ __forceinline__ bool page_at(const AttnArgs &a, const int32_t *table, uint32_t token, int32_t &page, int32_t *error_word) {
-    page = table[token / a.op.kv.page_tokens];
+// Page of a token for the copies, and its place there.
+__device__ __forceinline__ uint32_t page_index(const AttnArgs &a, uint32_t token) {
+    return (uint32_t)((unsigned long long)token * a.page_factor >> a.page_shift);
+}
+// Whether a table entry is a page; if not, the device error.
+__device__ __forceinline__ bool is_page(const AttnArgs &a, int32_t page, int32_t *error_word) {
     if (page >= 0 && (uint32_t)page < a.op.kv.n_pages) return true;
     bad_index(error_word);
     return false;
@@ -88,19 +113,28 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, u
         "l"(map), "r"(bar), "r"(0), "r"(chunk), "r"(group), "r"(step)
         : "memory");
 }
+// The same by either CTA of a pair into its own shared memory, complete at a barrier of the first (umma.cuh: tma_load_pair).
+__device__ __forceinline__ void load_box_pair(uint32_t dst, const CUtensorMap *map, uint32_t leader_bar, int chunk, int group, int step) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %3, %4, %5, %6}], [%2];" ::"r"(
+            dst),
+        "l"(map), "r"(leader_bar), "r"(0), "r"(chunk), "r"(group), "r"(step)
+        : "memory");
+}
 __device__ __forceinline__ int box_step(const AttnArgs &a, int32_t page, uint32_t head) {
     return (int)((uint32_t)page * a.pages_per_step + (a.op.kv_heads > 1 ? head : 0));
 }
 #endif
 
-// The cache as tensor maps: boxes of `box` tokens by chunks * 64 dimensions of one head. In shared memory eight tokens are
-// together, 128 bytes each, swizzled, chunk after chunk.
-ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attention_op &op, const void *base, uint32_t box, uint32_t chunks);
+// The cache as tensor maps: boxes of `box` tokens by `chunks` * `width` dimensions of one head (width 64, or 32). In shared memory eight
+// tokens are together, 2 * width bytes each, swizzled, chunk after chunk.
+ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attention_op &op, const void *base, uint32_t box, uint32_t chunks,
+                      uint32_t width = 64);
 
 // Requests with few rows (paged_attention.cu) and with many (paged_attention_tile.cu).
 ctox_status launch_attention_rows(ctox_ctx *ctx, AttnArgs &a);
 ctox_status launch_attention_tile(ctox_ctx *ctx, AttnArgs &a);
-uint32_t tile_block_rows(uint32_t dim);
+constexpr uint32_t kTileBlockRows = 256;  // of the latter's units
 
 }  // namespace paged
 }  // namespace ctox

@@ -1,67 +1,141 @@
 // Attention over a paged K/V cache for requests with many rows: pieces of prompts, whole prompts, long verify passes.
 //
-// The rows of a request and KV head, (token, query head) pairs in order, are cut into tiles of 128, so that one read of a key
-// serves all query heads that share it and a tile is full whatever their number. Scores S = Q K^T and the output O += P V run
-// on tcgen05 with accumulators in tensor memory; a thread owns a row for the softmax (running maximum and sum in
-// registers) and writes the weights P over its scores, where the next product takes them from. The output is rescaled only when a
-// row's maximum has grown by more than 2^8 since its last reference; the division at the end makes up for it.
+// The rows of a request and KV head, (token, query head) pairs in order, are cut into blocks of 256, so that one read of a key
+// serves all query heads that share it and a block is full whatever their number. A pair of CTAs takes a block, 128 rows each, and forms
+// scores S = Q K^T and output O += P V together on tcgen05: each keeps half of a key tile's keys and half of its values' dimensions in
+// shared memory, which halves what a CTA must fetch for its products (with 128 dimensions a CTA alone would want 64 bytes per cycle
+// from L2), and S, P and O of its own rows in tensor memory.
 //
-// Up to 128 dimensions a CTA works on two tiles of rows against the same keys: while the tensor cores form one tile's scores and
-// output, four warps each do the other's softmax, and a key tile in shared memory serves 256 rows. With 256 dimensions the output
-// of one tile fills half of tensor memory, and with one tile of rows there is only one: then even and odd key tiles take turns with
-// the two score buffers, so that the scores of the next key tile are formed while the softmax of this one runs.
+// Key tiles of 128 go round two or three score buffers and, in turn, to two groups of four softmax warps (a thread owns a row), so that the
+// tensor cores always have the next scores to form while both groups work. The weights of a row are taken against a reference that is
+// its maximum over the first tile that it sees, and stays: weights that then exceed 1 cost nothing in a floating-point format. Only when a
+// tile's weights add up to more than 2^60 (f16: 2^15) is the reference raised and the output rescaled; the division at the end
+// makes up for it either way. So after the first tile no maximum is formed and no tile waits for the one before, but for the
+// news that the reference has not changed.
 #include "paged_attention.cuh"
 #include "f32x2.cuh"
+
+#include <type_traits>
 
 namespace ctox {
 namespace paged {
 namespace {
 
 constexpr uint32_t kTileRows = 128, kTileKeys = 128, kTileThreads = 384;
-constexpr uint32_t kLoadWarp = 8, kIssueWarp = 9, kMostSlots = 8;
+constexpr uint32_t kLoadWarp = 8, kIssueWarp = 9, kClearWarp = 10, kMostSlots = 8;
 // Registers: twelve warps are launched with 168 each. The softmax warps hold a row of 128 scores and take 208; the four others (copies,
-// products, two without work) keep 88: 8 * 208 + 4 * 88 = 12 * 168.
+// products, clearing, one without work) keep 88: 8 * 208 + 4 * 88 = 12 * 168.
 constexpr uint32_t kSoftmaxRegisters = 208, kOtherRegisters = 88;
 
 template <int D>
 struct Tile {
-    static constexpr uint32_t NQ = D == 256 ? 1 : 2;      // tiles of rows
-    static constexpr uint32_t CH = D == 64 ? 1 : 2;       // chunks of 64 dimensions in a slot of the ring
-    static constexpr uint32_t HALVES = D == 256 ? 2 : 1;  // slots of a key tile, and of its values
-    static constexpr uint32_t SLOT = kTileKeys * CH * 128;
+    static constexpr uint32_t NB = D == 256 ? 2 : 3;            // score buffers: what tensor memory holds beside the output
+    static constexpr uint32_t SLOT = 128 * D;                   // of the ring: 64 keys, or half the dimensions of 128 values
     static constexpr uint32_t Q_BYTES = kTileRows * D * 2;
-    static constexpr uint32_t N_O = D < 128 ? D : 128;  // columns of a product with values
+    static constexpr uint32_t VW = D == 64 ? 32 : 64;           // dimensions in a swizzled row of a value tile
+    static constexpr uint32_t VC = D / 2 / VW;                  // chunks of them in this CTA's half
+    static constexpr uint32_t V_GROUP = 8 * VW * 2 * VC;        // bytes of eight values
+    static constexpr uint32_t O = 0, S = D == 256 ? 256 : 128;  // columns of tensor memory
     static uint32_t slots(size_t room, uint32_t n) {
-        const size_t left = room - 1024 - NQ * Q_BYTES - (n + 1) * 8;
-        const uint32_t s = (uint32_t)(left / SLOT);
+        const uint32_t s = (uint32_t)((room - 1024 - Q_BYTES - (n + 1) * 8) / SLOT);
         return s < kMostSlots ? s : kMostSlots;
     }
-    static size_t smem(uint32_t slots, uint32_t n) { return 1024 + NQ * Q_BYTES + (size_t)slots * SLOT + (n + 1) * 8; }
+    static size_t smem(uint32_t slots, uint32_t n) { return 1024 + Q_BYTES + (size_t)slots * SLOT + (n + 1) * 8; }
 };
 
-// Place in the ring's order of the keys (values) of tile j of n. Two tiles of rows need K0 V0 K1 V1 ..., one needs K0 K1 V0 K2 V1 ...
-__device__ __forceinline__ uint32_t key_place(bool two, uint32_t j) { return two ? 2 * j : j < 2 ? j : 2 * j - 1; }
-__device__ __forceinline__ uint32_t value_place(bool two, uint32_t j, uint32_t n) { return two ? 2 * j + 1 : j + 1 < n ? 2 * j + 2 : 2 * n - 1; }
-
 template <typename T>
-__host__ __device__ constexpr uint32_t idesc(uint32_t n, bool b_mn);
+struct Weights;
 template <>
-__host__ __device__ constexpr uint32_t idesc<__nv_bfloat16>(uint32_t n, bool b_mn) {
-    return umma::idesc_bf16_mn(kTileRows, n, false, b_mn);
-}
+struct Weights<__nv_bfloat16> {
+    static constexpr float limit = 1152921504606846976.f;  // 2^60
+    // 2^f over [-1/2, 1/2] as 1 + f (c1 + f (c2 + ...)): largest relative error 1.0e-4, against 2^-9 of a weight's rounding
+    static constexpr int terms = 3;
+    __device__ static constexpr float c(int i) { return i == 0 ? 0.6932829022407532f : i == 1 ? 0.2422109693288803f : 0.05500893294811249f; }
+    __host__ __device__ static constexpr uint32_t idesc(uint32_t n, bool b_mn) { return umma::idesc_bf16_mn(2 * kTileRows, n, false, b_mn); }
+};
 template <>
-__host__ __device__ constexpr uint32_t idesc<__half>(uint32_t n, bool b_mn) {
-    return umma::idesc_bf16_mn(kTileRows, n, false, b_mn) & ~((1u << 7) | (1u << 10));  // the types' fields: 0 for f16
+struct Weights<__half> {
+    static constexpr float limit = 32768.f;  // no weight above the type's 65504
+    // the same with 2.9e-6, against 2^-12
+    static constexpr int terms = 4;
+    __device__ static constexpr float c(int i) {
+        return i == 0 ? 0.6931241750717163f : i == 1 ? 0.24024099111557007f : i == 2 ? 0.055906426161527634f : 0.009582852944731712f;
+    }
+    __host__ __device__ static constexpr uint32_t idesc(uint32_t n, bool b_mn) {
+        return Weights<__nv_bfloat16>::idesc(n, b_mn) & ~((1u << 7) | (1u << 10));  // the types' fields: 0 for f16
+    }
+};
+
+// 2^x of two values without the special-function unit, which has 16 lanes per cycle for 128 rows of 128 scores: the pipes
+// for multiplications take a quarter of them. x is cut into a whole number (added to 1.5 * 2^23 it is in the low bits) and the rest
+// in [-1/2, 1/2], for which a polynomial, fitted for the least largest relative error, is near enough to what the type keeps; the
+// whole number then goes into the exponent. Below 2^-127 the result is 0, exactly: there the polynomial is 1. From 2^127 on it is 2^127,
+// and what is no number stays none or becomes large: either makes the tile's sum too large, and the tile is formed again by ex2.
+__device__ __forceinline__ float clamp_exponent(float x) {
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n\tmin.NaN.f32 %0, %0, 0f42FE0000;" : "+f"(x));  // -127, 127
+    return x;
 }
-// Operands of 128-byte swizzled rows: `group` bytes from eight rows (keys) to the next eight; keys run along m or n, or along k
-// with `atom` bytes from 64 dimensions to the next.
+template <typename T>
+__device__ __forceinline__ void exp2_pair(f32x2 v, float &a, float &b) {
+    using W = Weights<T>;
+    unpack2(v, a, b);
+    v = pack2(clamp_exponent(a), clamp_exponent(b));
+    const f32x2 one = pack2(1.f, 1.f), magic = pack2(12582912.f, 12582912.f), minus_magic = pack2(-12582912.f, -12582912.f),
+                minus_one = pack2(-1.f, -1.f);
+    const f32x2 t = fma2(v, one, magic);  // rounds to a whole number
+    const f32x2 f = fma2(fma2(t, one, minus_magic), minus_one, v);
+    f32x2 y = pack2(W::c(W::terms - 1), W::c(W::terms - 1));
+#pragma unroll
+    for (int i = W::terms - 2; i >= 0; --i) y = fma2(y, f, pack2(W::c(i), W::c(i)));
+    y = fma2(y, f, one);
+    float ta, tb;
+    unpack2(t, ta, tb);
+    unpack2(y, a, b);
+    a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
+    b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
+}
+
+// Operands of swizzled rows of `width` bytes: `group` bytes from eight rows (keys) to the next eight; keys run along n (128 bytes), or along
+// k with `atom` bytes from a row's dimensions to the next ones.
 __device__ __forceinline__ uint64_t desc_rows(uint32_t addr, uint32_t group) {
     return (uint64_t)((addr & 0x3ffff) >> 4) | (1ull << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ uint64_t desc_columns(uint32_t addr, uint32_t group, uint32_t atom) {
-    return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(atom >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ uint64_t desc_columns(uint32_t addr, uint32_t width, uint32_t group, uint32_t atom) {
+    return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(atom >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) |
+           ((width == 128 ? 2ull : 4ull) << 61);
+}
+// The compiler forms these before the next load from tensor memory: left to itself it puts them off until four loads are live, and spills.
+__device__ __forceinline__ void keep16(uint32_t *p, f32x2 (&sums)[2]) {
+    asm volatile("" : "+r"(p[0]), "+r"(p[1]), "+r"(p[2]), "+r"(p[3]), "+r"(p[4]), "+r"(p[5]), "+r"(p[6]), "+r"(p[7]), "+r"(p[8]), "+r"(p[9]), "+r"(p[10]),
+                 "+r"(p[11]), "+r"(p[12]), "+r"(p[13]), "+r"(p[14]), "+r"(p[15]), "+l"(sums[0]), "+l"(sums[1]));
 }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void store16(uint32_t addr, uint4 x) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+}
+__device__ __forceinline__ uint4 load16(uint32_t addr) {
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(addr) : "memory");
+    return x;
+}
+
+// Barriers, 8 bytes each. A tile has the number n in the order of all tiles of the CTA; with n % 6 the barrier belongs to one score buffer
+// and one group of warps, so that whoever waits meets every phase of it.
+enum : uint32_t {
+    B_FULL = 0,                        // ring, at the first CTA: both CTAs' copies
+    B_EMPTY = B_FULL + kMostSlots,     // both CTAs: the products have read a slot
+    B_LOCAL = B_EMPTY + kMostSlots,    // this CTA's copies of a value tile that is cleared in part
+    B_CLEAR = B_LOCAL + kMostSlots,    // at the first CTA: cleared, by both
+    B_S = B_CLEAR + kMostSlots,        // [6] both CTAs: scores
+    B_P = B_S + 6,                     // [6] at the first CTA: weights, by four warps of each
+    B_REF = B_P + 6,                   // [4 quarters][2]: the reference is settled for tile n, by its warp
+    B_SUM = B_REF + 8,                 // [4 quarters]: both groups' sums
+    B_PV = B_SUM + 4,                  // [2] both CTAs: output of tile n
+    B_Q = B_PV + 2,                    // at the first CTA: queries, by eight warps of each
+    B_END = B_Q + 1,                   // both CTAs: the unit's products
+    B_DRAINED = B_END + 1,
+    B_COUNT = B_DRAINED + 1
+};
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -70,364 +144,553 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     using namespace umma;
     using G = Tile<D>;
     extern __shared__ uint8_t raw[];
-    // ring; queries of each tile of rows; scores and weights of score buffer 0, of buffer 1 when it is the second tile's, and of
-    // buffer 1 when it is the first's; end of a unit for each tile of rows; products with values that a rescale waits for
-    __shared__ __align__(8) uint64_t bars[2 * kMostSlots + 2 + 3 + 3 + 2 + 2 + 1];
+    __shared__ __align__(8) uint64_t bars[B_COUNT];
     __shared__ unsigned long long scan[32];
+    __shared__ float refs[kTileRows], sums_of[2][kTileRows];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
     __shared__ Cut cuts[2];
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t base = (smem_addr(raw) + 1023) & ~1023u, q_s = base, ring = q_s + G::NQ * G::Q_BYTES;
+    __shared__ Walk walks[8];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster_rank(), piece = blockIdx.x >> 1;
+    const uint32_t base = (smem_addr(raw) + 1023) & ~1023u, q_s = base, ring = q_s + G::Q_BYTES;
     unsigned long long *at = reinterpret_cast<unsigned long long *>(raw + (ring + slots * G::SLOT - smem_addr(raw)));
-    const uint32_t full = smem_addr(bars), empty = full + kMostSlots * 8, q_full = empty + kMostSlots * 8, s_full = q_full + 16,
-                   p_full = s_full + 24, fin = p_full + 24, o_done = fin + 16, drained = o_done + 16;
+    const uint32_t b0 = smem_addr(bars);
+    auto bar = [&](uint32_t i) { return b0 + i * 8; };
     if (tid == 0) {
         dead = 0;
-        for (uint32_t i = 0; i < slots; ++i) {
-            bar_init(full + i * 8, 1);
-            bar_init(empty + i * 8, 1);
+        for (uint32_t i = 0; i < kMostSlots; ++i) {
+            bar_init(bar(B_FULL + i), 1);
+            bar_init(bar(B_EMPTY + i), 1);
+            bar_init(bar(B_LOCAL + i), 1);
+            bar_init(bar(B_CLEAR + i), 2);
         }
-        for (uint32_t i = 0; i < 2; ++i) {
-            bar_init(q_full + i * 8, 4);
-            bar_init(fin + i * 8, 1);
-            bar_init(o_done + i * 8, 1);
+        for (uint32_t i = 0; i < 6; ++i) {
+            bar_init(bar(B_S + i), 1);
+            bar_init(bar(B_P + i), 8);
         }
-        for (uint32_t i = 0; i < 3; ++i) {
-            bar_init(s_full + i * 8, 1);
-            bar_init(p_full + i * 8, 4);
-        }
-        bar_init(drained, 1);
+        for (uint32_t i = 0; i < 8; ++i) bar_init(bar(B_REF + i), 1);
+        for (uint32_t i = 0; i < 4; ++i) bar_init(bar(B_SUM + i), 2);
+        bar_init(bar(B_PV), 1);
+        bar_init(bar(B_PV + 1), 1);
+        bar_init(bar(B_Q), 16);
+        bar_init(bar(B_END), 1);
+        bar_init(bar(B_DRAINED), 1);
         bar_init_fence();
     }
-    if (warp == kIssueWarp) tmem_alloc(smem_addr(&tmem_slot), 512);
+    if (warp == kIssueWarp) tmem_alloc_pair(smem_addr(&tmem_slot), 512);
     fence_before();
     __syncthreads();
+    cluster_sync();  // the other CTA's barriers are ready
     fence_after();
     const uint32_t tmem = tmem_slot;
     pdl_launch();
     pdl_wait();
-    const uint64_t total = lay_line(a, at, scan, error_word);
-    const uint32_t pieces = total ? pieces_of(total, gridDim.x, a.least) : 0;
+    lay_line(a, at, scan, reinterpret_cast<uint32_t *>(raw), error_word);
     const Line line{a, at, a.op.n_requests};
+    const Cuts cut = cuts_of(at[a.op.n_requests], gridDim.x >> 1, a.least);
     Walk w;
     w.at.x = w.end = 0;
-    if (blockIdx.x < pieces) {
+    if (piece < cut.pieces) {
         if (warp < 2) {
-            const Cut c = cut_at(a.shape, line, total, pieces, blockIdx.x + warp, a.least);
+            const Cut c = cut_at(a.shape, line, cut, piece + warp);
             if (lane == 0) cuts[warp] = c;
         }
         __syncthreads();
         w.at = cuts[0];
         w.end = cuts[1].x;
     }
+    // a value tile with places that no row of the unit sees, which may hold anything
+    auto is_edge = [&](uint32_t j) {
+        const uint32_t key0 = (w.u.tile0 + w.tile0 + j) * kTileKeys;
+        return key0 < w.u.lo || key0 + kTileKeys > w.u.hi;
+    };
     bool ok = true;
     if (warp >= kLoadWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
         if (warp == kLoadWarp) {
-            const uint32_t per = kTileKeys / a.box, box_bytes = a.box * G::CH * 128;
-            uint32_t n = 0;  // slots filled
+            // A lane per box of a key tile; the CTAs take the boxes of 64 keys each, and half the dimensions of all values.
+            const uint32_t boxes = kTileKeys / a.box, k_bytes = a.box * D * 2, v_bytes = a.box * D;
+            uint32_t n = 0, slot = 0, round = 0;  // slots filled, and where that leaves the ring
             for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
                 const int32_t *table = table_row(a, w.at.request);
-                const bool two = w.u.rows > kTileRows;
-                const uint32_t tiles = w.tile1 - w.tile0;
-                uint32_t kj = 0, vj = 0;  // the next tile of each
-                for (uint32_t i = 0; ok && i < 2 * tiles; ++i) {
-                    const bool is_k = kj < tiles && key_place(two, kj) == i;
-                    const uint32_t j = is_k ? kj++ : vj++;
-                    const uint32_t token = (w.u.tile0 + w.tile0 + j) * kTileKeys + lane * a.box;
-                    int32_t page = -1;
-                    bool mine = lane < per && token < w.u.hi && token + a.box > w.u.lo;
-                    if (mine) mine = page_at(a, table, token, page, error_word);
-                    const uint32_t copies = __popc(__ballot_sync(0xffffffffu, mine));
-                    for (uint32_t h = 0; h < G::HALVES; ++h, ++n) {
-                        const uint32_t s = n % slots, round = n / slots;
-                        if (round > 0 && !(ok = __all_sync(0xffffffffu, bar_wait(empty + s * 8, (round - 1) & 1, &dead)))) break;
-                        if (lane == 0) bar_expect(full + s * 8, copies * box_bytes);
-                        __syncwarp();
-                        if (mine)
-                            load_box(ring + s * G::SLOT + lane * box_bytes, is_k ? &map_k : &map_v, full + s * 8, (int)(h * G::CH),
-                                     (int)(token % a.op.kv.page_tokens / 8), box_step(a, page, w.at.head));
-                    }
-                }
-            }
-            if (!ok && lane == 0)  // leave no copy in flight behind
-                for (uint32_t s = 0; s < slots && s < n; ++s) bar_drain(full + s * 8, ((n - 1 - s) / slots) & 1);
-        } else if (warp == kIssueWarp) {
-            constexpr uint32_t idesc_s = idesc<T>(kTileKeys, false), idesc_o = idesc<T>(G::N_O, true);
-            const bool leader = elect_one();  // one thread throughout: a commit covers what its own thread issued
-            uint32_t ring0 = 0, units[2] = {0, 0}, weights[3] = {0, 0, 0};
-            for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
-                const bool two = w.u.rows > kTileRows;
-                const uint32_t tiles = w.tile1 - w.tile0, steps = two ? 2 * tiles : tiles;
-                if (!tiles) continue;
-                auto slot_full = [&](uint32_t place, uint32_t h) {
-                    const uint32_t n = ring0 + place * G::HALVES + h;
-                    return __all_sync(0xffffffffu, bar_wait(full + n % slots * 8, (n / slots) & 1, &dead));
+                const uint32_t tiles = w.tile1 - w.tile0, first = (w.u.tile0 + w.tile0) * kTileKeys + lane * a.box;
+                // Order of the ring: the keys of as many tiles as there are score buffers, then values and keys in turn. `entry`: this lane's page
+                // of a tile, INT32_MIN where no row sees what its box holds. Entries of the table are read one tile ahead.
+                auto entry = [&](uint32_t j) {
+                    const uint32_t token = first + j * kTileKeys;
+                    return j < tiles && lane < boxes && token < w.u.hi && token + a.box > w.u.lo ? table[page_index(a, token)] : INT32_MIN;
                 };
-                auto slot_of = [&](uint32_t place, uint32_t h) { return (ring0 + place * G::HALVES + h) % slots; };
-                auto scores = [&](uint32_t i) {
-                    const uint32_t j = two ? i >> 1 : i, t = two ? i & 1 : 0, place = key_place(two, j);
-                    for (uint32_t h = 0; h < G::HALVES; ++h)
-                        if (!slot_full(place, h)) return false;
-                    fence_after();
-                    if (leader) {
-                        uint64_t dq = desc_rows(q_s + t * G::Q_BYTES, 1024);
-#pragma unroll
-                        for (uint32_t h = 0; h < G::HALVES; ++h) {
-                            uint64_t dk = desc_rows(ring + slot_of(place, h) * G::SLOT, G::CH * 1024);
-                            asm volatile("" : "+l"(dq), "+l"(dk));  // formed here, not kept for the whole unit
-#pragma unroll
-                            for (uint32_t k = 0; k < G::CH * 4; ++k)
-                                mma_f16(tmem + (i & 1) * kTileKeys, dq + ((h * G::CH + k / 4) * (kTileRows * 128) + k % 4 * 32) / 16,
-                                        dk + (k / 4 * 1024 + k % 4 * 32) / 16, idesc_s, h > 0 || k > 0);
+                auto load = [&](bool keys, uint32_t j, int32_t page) {
+                    const bool mine = page != INT32_MIN && is_page(a, page, error_word);
+                    const uint32_t copies = __popc(__ballot_sync(0xffffffffu, mine)), token = first + j * kTileKeys;
+                    const int group = (int)((token - page_index(a, token) * a.op.kv.page_tokens) / 8);
+                    const bool edge = !keys && is_edge(j);
+                    if (round > 0 && !(ok = __all_sync(0xffffffffu, bar_wait(bar(B_EMPTY + slot), (round - 1) & 1, &dead)))) return;
+                    const uint32_t full = bar(B_FULL + slot), dst = ring + slot * G::SLOT;
+                    if (lane == 0) {
+                        if (edge) bar_expect(bar(B_LOCAL + slot), copies * v_bytes);
+                        if (rank == 0) {  // both CTAs' bytes: for keys and for values a box has as many
+                            if (edge)
+                                bar_arrive(full);
+                            else
+                                bar_expect(full, copies * k_bytes);
                         }
-                        commit(s_full + (two ? i & 1 : (i & 1) * 2) * 8);
-                        if (!two || t == 1)
-                            for (uint32_t h = 0; h < G::HALVES; ++h) commit(empty + slot_of(place, h) * 8);
                     }
                     __syncwarp();
-                    return true;
+                    const int step = box_step(a, page, w.at.head);
+                    if (mine && keys && lane / (boxes / 2) == rank)
+                        load_box_pair(dst + lane % (boxes / 2) * k_bytes, &map_k, leader_addr(full), 0, group, step);
+                    if (mine && !keys) {
+                        if (edge)
+                            load_box(dst + lane * v_bytes, &map_v, bar(B_LOCAL + slot), (int)(rank * G::VC), group, step);
+                        else
+                            load_box_pair(dst + lane * v_bytes, &map_v, leader_addr(full), (int)(rank * G::VC), group, step);
+                    }
+                    ++n;
+                    if (++slot == slots) {
+                        slot = 0;
+                        ++round;
+                    }
                 };
-                ok = __all_sync(0xffffffffu, bar_wait(q_full, units[0] & 1, &dead) && (!two || bar_wait(q_full + 8, units[1] & 1, &dead)));
-                ++units[0];
-                if (two) ++units[1];
-                fence_after();
-                ok = ok && scores(0) && (steps < 2 || scores(1));
-                for (uint32_t i = 0; ok && i < steps; ++i) {
-                    const uint32_t j = two ? i >> 1 : i, t = two ? i & 1 : 0, b = two ? i & 1 : (i & 1) * 2, place = value_place(two, j, tiles);
-                    if (!(ok = __all_sync(0xffffffffu, bar_wait(p_full + b * 8, weights[b] & 1, &dead)))) break;
-                    ++weights[b];
-                    for (uint32_t h = 0; ok && h < G::HALVES; ++h) ok = slot_full(place, h);
-                    if (!ok) break;
-                    const uint32_t key0 = (w.u.tile0 + w.tile0 + j) * kTileKeys;
-                    if (t == 0 && (key0 < w.u.lo || key0 + kTileKeys > w.u.hi)) {
-                        // values in places that no row sees may be anything, and 0 times that is not 0
-                        for (uint32_t r = 0; r < kTileKeys; ++r) {
-                            if (key0 + r >= w.u.lo && key0 + r < w.u.hi) continue;
-                            for (uint32_t h = 0; h < G::HALVES; ++h)
-                                if (lane < G::CH * 8)
-                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + slot_of(place, h) * G::SLOT +
-                                                                                                  (r >> 3) * (G::CH * 1024) + (lane >> 3) * 1024 +
-                                                                                                  (r & 7) * 128 + (lane & 7) * 16),
-                                                 "r"(0)
-                                                 : "memory");
-                        }
-                        proxy_fence();
-                        __syncwarp();
-                    }
-                    fence_after();
-                    if (leader) {
+                // pages of the tile whose values are next and of those behind it
+                int32_t page[G::NB + 1];
 #pragma unroll
-                        for (uint32_t h = 0; h < G::HALVES; ++h) {
-                            uint64_t dv = desc_columns(ring + slot_of(place, h) * G::SLOT, G::CH * 1024, 1024);
-                            asm volatile("" : "+l"(dv));
+                for (uint32_t i = 0; i <= G::NB; ++i) page[i] = entry(i);
 #pragma unroll
-                            for (uint32_t k = 0; k < kTileKeys / 16; ++k)
-                                mma_f16_ts(tmem + 256 + t * D + h * 128, tmem + (i & 1) * kTileKeys + k * 8, dv + k * (2 * G::CH * 1024 / 16), idesc_o,
-                                           j > 0 || k > 0);
-                        }
-                        if (!two || t == 1)
-                            for (uint32_t h = 0; h < G::HALVES; ++h) commit(empty + slot_of(place, h) * 8);
-                        if (!two) commit(o_done + (i & 1) * 8);
-                        if (j + 1 == tiles) commit(fin + t * 8);
-                    }
-                    __syncwarp();
-                    if (i + 2 < steps) ok = scores(i + 2);
+                for (uint32_t i = 0; i < G::NB; ++i)
+                    if (ok && i < tiles) load(true, i, page[i]);
+                for (uint32_t v = 0; ok && v < tiles; ++v) {
+                    load(false, v, page[0]);
+                    if (ok && v + G::NB < tiles) load(true, v + G::NB, page[G::NB]);
+#pragma unroll
+                    for (uint32_t i = 0; i < G::NB; ++i) page[i] = page[i + 1];
+                    page[G::NB] = entry(v + 1 + G::NB);
                 }
-                ring0 += 2 * tiles * G::HALVES;
             }
-            if (!ok) {
-                if (leader) commit(drained);
+            if (!ok) {  // leave no copy in flight behind; the barriers may lack the other CTA's part, so by time
+                const long long t0 = clock64();
+                while (clock64() - t0 < 2000000) {
+                }
+            }
+        } else if (warp == kIssueWarp && rank == 0) {
+            // the whole warp runs the loop and one lane issues: its values are uniform
+            constexpr uint32_t idesc_s = Weights<T>::idesc(kTileKeys, false), idesc_o = Weights<T>::idesc(D, true);
+            const bool issuer = elect_one();
+            uint32_t next = 0, next_phase = 0, cleared = 0;  // of the ring; phases of B_CLEAR
+            uint32_t units = 0, s6 = 0, p6 = 0, p6_phase = 0, buffer_s = 0, buffer_p = 0, pv = 0;
+            auto take = [&](bool edge) {  // the next slot, once it is full
+                const uint32_t slot = next;
+                ok = ok && __all_sync(0xffffffffu, bar_wait(bar(B_FULL + slot), next_phase, &dead));
+                if (edge) {
+                    ok = ok && __all_sync(0xffffffffu, bar_wait<BAR_PAIR>(bar(B_CLEAR + slot), cleared >> slot & 1, &dead));
+                    cleared ^= 1u << slot;
+                }
+                if (++next == slots) {
+                    next = 0;
+                    next_phase ^= 1;
+                }
+                return slot;
+            };
+            auto scores = [&](uint32_t slot) {  // S = Q K^T of the next tile
+                if (issuer) {
+                    const uint64_t dq = desc_rows(q_s, 1024), dk = desc_rows(ring + slot * G::SLOT, D * 16);
+                    const uint32_t d = tmem + G::S + buffer_s * kTileKeys;
+#pragma unroll
+                    for (uint32_t k = 0; k < D / 16; ++k)
+                        mma_f16_pair(d, dq + (k / 4 * (kTileRows * 128) + k % 4 * 32) / 16, dk + (k / 4 * 1024 + k % 4 * 32) / 16, idesc_s, k > 0);
+                    commit_pair(bar(B_S + s6));
+                    commit_pair(bar(B_EMPTY + slot));
+                }
                 __syncwarp();
-                bar_drain(drained, 0);
+                s6 = s6 == 5 ? 0 : s6 + 1;
+                buffer_s = buffer_s + 1 == G::NB ? 0 : buffer_s + 1;
+            };
+            for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
+                const uint32_t tiles = w.tile1 - w.tile0;
+                if (!tiles) continue;
+                if (!(ok = __all_sync(0xffffffffu, bar_wait<BAR_PAIR>(bar(B_Q), units++ & 1, &dead)))) break;
+                for (uint32_t j = 0; ok && j < G::NB && j < tiles; ++j) {
+                    const uint32_t slot = take(false);
+                    fence_after();
+                    if (ok) scores(slot);
+                }
+                for (uint32_t j = 0; ok && j < tiles; ++j) {  // O += P V
+                    // both operands are there long before the weights
+                    const uint32_t slot = take(is_edge(j)), keys = j + G::NB < tiles ? take(false) : 0;
+                    ok = ok && __all_sync(0xffffffffu, bar_wait<BAR_PAIR_TURN>(bar(B_P + p6), p6_phase, &dead));
+                    if (!ok) break;
+                    fence_after();
+                    if (issuer) {
+                        const uint64_t dv = desc_columns(ring + slot * G::SLOT, G::VW * 2, G::V_GROUP, G::VW * 16);
+                        const uint32_t p = tmem + G::S + buffer_p * kTileKeys;
+#pragma unroll
+                        for (uint32_t k = 0; k < kTileKeys / 16; ++k)
+                            mma_f16_ts_pair(tmem + G::O, p + k * 8, dv + k * (2 * G::V_GROUP / 16), idesc_o, j > 0 || k > 0);
+                        commit_pair(bar(B_EMPTY + slot));
+                        commit_pair(bar(B_PV + (pv & 1)));
+                        if (j + 1 == tiles) commit_pair(bar(B_END));
+                    }
+                    __syncwarp();
+                    ++pv;
+                    buffer_p = buffer_p + 1 == G::NB ? 0 : buffer_p + 1;
+                    if (++p6 == 6) {
+                        p6 = 0;
+                        p6_phase ^= 1;
+                    }
+                    if (j + G::NB < tiles) scores(keys);
+                }
+            }
+            if (!ok && issuer) {
+                commit_pair(bar(B_DRAINED));
+                bar_drain(bar(B_DRAINED), 0);
+            }
+            __syncwarp();
+        } else if (warp == kClearWarp) {
+            // 0 times what lies in places that no row sees is not 0 if that is no number
+            uint32_t ring0 = 0, local = 0;  // slots before the unit; phases of B_LOCAL
+            for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
+                const uint32_t tiles = w.tile1 - w.tile0;
+                for (uint32_t j = 0; j < tiles; ++j) {
+                    if (!is_edge(j)) continue;
+                    const uint32_t slot = (ring0 + min(min(G::NB, tiles) + j, tiles) + j) % slots, key0 = (w.u.tile0 + w.tile0 + j) * kTileKeys;
+                    const uint32_t x = w.u.lo > key0 ? w.u.lo - key0 : 0, y = min(w.u.hi - key0, kTileKeys);  // rows [x, y) stay
+                    if (!(ok = __all_sync(0xffffffffu, bar_wait(bar(B_LOCAL + slot), local >> slot & 1, &dead)))) break;
+                    local ^= 1u << slot;
+                    constexpr uint32_t pieces = D / 16;  // of 16 bytes in a row: four rows of 128, eight of 64 and two of 256 dimensions at a time
+                    for (uint32_t r = lane / pieces; r < kTileKeys; r += 32 / pieces) {
+                        const uint32_t i = lane % pieces, chunk = i / (G::VW / 8), in = i % (G::VW / 8);
+                        if (r < x || r >= y)
+                            store16(ring + slot * G::SLOT + (r >> 3) * G::V_GROUP + chunk * (G::VW * 16) + (r & 7) * (G::VW * 2) + in * 16,
+                                    make_uint4(0, 0, 0, 0));
+                    }
+                    proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) bar_release_leader(leader_addr(bar(B_CLEAR + slot)));
+                }
+                ring0 += 2 * tiles;
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-        const uint32_t t = warp >> 2, row = tid & 127, lanes = ((warp & 3) * 32) << 16;  // tile of rows, row in it
+        const uint32_t g = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, lanes = (quarter * 32) << 16;
+        const uint32_t in = rank * kTileRows + row;  // of the unit's rows
+        constexpr uint32_t P = D / 16, ROWS = 32 / P;  // 16-byte pieces of half a row; rows that a warp moves at a time
         const float c = a.c;
+        const f32x2 cc = pack2(c, c), one = pack2(1.f, 1.f);
         bool shares = false;
-        uint32_t units = 0, seen[2] = {0, 0}, done[2] = {0, 0};
-        for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
-            const bool two = w.u.rows > kTileRows;
-            const uint32_t tiles = w.tile1 - w.tile0, group = a.shape.group;
-            if (w.begins && !w.ends) {
-                shares = true;
-                if (tid == 0)
-                    a.shared[blockIdx.x] = Shared{sharers(total, pieces, blockIdx.x, w.at.start + w.u.cost), w.at.request, w.at.head, w.u.row0, w.u.rows};
+        uint32_t units = 0, n = 0, n6 = 0, n6_phase = 0, nb = 0;  // tiles so far, modulo 6 with its phase, modulo the buffers
+        auto next_tile = [&]() {
+            ++n;
+            nb = nb + 1 == G::NB ? 0 : nb + 1;
+            if (++n6 == 6) {
+                n6 = 0;
+                n6_phase ^= 1;
             }
-            const uint32_t in = t * kTileRows + row, r = w.u.row0 + in;
-            const bool live = in < w.u.rows;
-            const uint32_t token = w.q.q0 + r / group, head = w.at.head * group + r % group;
+        };
+        auto settled = [&](uint32_t tile) { return bar_wait(bar(B_REF + quarter * 2 + (tile & 1)), tile >> 1 & 1, &dead); };
+        // Where the walk stands is kept in shared memory, one for each warp: in registers it would push scores out of them.
+        Walk &u = walks[warp];
+        if (lane == 0) u = w;
+        for (bool first = true; ok; first = false) {
+            __syncwarp();
+            bool more = true;
+            if (lane == 0) {
+                if (!first) walk_on(a.shape, line, u);
+                more = walk_unit(a.shape, line, u);
+            }
+            if (!__shfl_sync(0xffffffffu, more, 0)) break;
+            __syncwarp();
+            const uint32_t tiles = u.tile1 - u.tile0;
+            const bool whole_unit = u.begins && u.ends;
+            if (u.begins && !u.ends) {
+                shares = true;
+                if (tid == 0 && rank == 0)
+                    a.shared[piece] = Shared{sharers(cut, piece, u.at.start + u.u.cost), u.at.request, u.at.head, u.u.row0, u.u.rows};
+            }
+            const bool live = in < u.u.rows;
+            const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
+            // this lane's row of q (or out), this group's half of its dimensions
+            auto row_of = [&](const void *m, uint64_t token_stride, uint64_t head_stride) {
+                const uint32_t r = u.u.row0 + in, t = r / a.shape.group;
+                return (unsigned long long)((const T *)m + (uint64_t)(u.q.q0 + t) * token_stride +
+                                            (uint64_t)(u.at.head * a.shape.group + (r - t * a.shape.group)) * head_stride + g * (D / 2));
+            };
+            // this warp's half (g) of its 32 rows: a piece of 16 bytes per lane, neighbours in a row by neighbouring lanes
+            uint32_t here = q_s;
+            asm volatile("" : "+r"(here));  // addresses formed where they are used, not kept through the tiles
+            auto piece_of = [&](uint32_t i, uint32_t &at_row) {
+                at_row = i * ROWS + lane / P;
+                const uint32_t col = g * P + lane % P, rr = quarter * 32 + at_row;
+                return here + (col >> 3) * (kTileRows * 128) + rr * 128 + (((col & 7) ^ (rr & 7)) << 4);
+            };
             float ref = -INFINITY;
-            f32x2 sums[2] = {0, 0};
-            if (tiles && (t == 0 || two)) {
+            f32x2 sums = 0;
+            if (tiles) {
                 {  // queries; the products of the unit before have finished
-                    const uint4 *q = reinterpret_cast<const uint4 *>((const T *)a.op.q + (uint64_t)token * a.op.q_token_stride +
-                                                                     (uint64_t)head * a.op.q_head_stride);
-                    const uint32_t d = q_s + t * G::Q_BYTES + row * 128;
+                    const unsigned long long q = row_of(a.op.q, a.op.q_token_stride, a.op.q_head_stride);
+                    constexpr uint32_t at_once = P < 8 ? P : 8;
+#pragma unroll 1
+                    for (uint32_t i0 = 0; i0 < P; i0 += at_once) {
+                        uint4 x[at_once];
 #pragma unroll
-                    for (uint32_t i = 0; i < D / 8; ++i) {
-                        const uint4 x = live ? q[i] : make_uint4(0, 0, 0, 0);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(d + i / 8 * (kTileRows * 128) + ((i % 8 ^ (row & 7)) << 4)),
-                                     "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
-                                     : "memory");
+                        for (uint32_t i = 0; i < at_once; ++i) {
+                            const uint32_t from = (i0 + i) * ROWS + lane / P;
+                            const T *src = (const T *)__shfl_sync(0xffffffffu, q, from);
+                            x[i] = live_rows >> from & 1 ? reinterpret_cast<const uint4 *>(src)[lane % P] : make_uint4(0, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < at_once; ++i) {
+                            uint32_t at_row;
+                            const uint32_t d = piece_of(i0 + i, at_row);
+                            store16(d, x[i]);
+                        }
                     }
                     proxy_fence();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(q_full + t * 8);
+                    if (lane == 0) bar_release_leader(leader_addr(bar(B_Q)));
                 }
                 uint32_t lo = 0, hi = 0;
-                if (live) key_range(a.shape, w.q, r, r + 1, lo, hi);
-                const bool idle = !__any_sync(0xffffffffu, live);
-                for (uint32_t j = 0; j < tiles; ++j) {
-                    const uint32_t buf = two ? t : j & 1, b = two ? t : (j & 1) * 2, o = j & 1;  // score buffer, its barriers
-                    uint32_t &phase = seen[!two && o];
-                    if (!(ok = __all_sync(0xffffffffu, bar_wait(s_full + b * 8, phase & 1, &dead)))) break;
-                    ++phase;
-                    fence_after();
-                    if (!idle) {
-                        float s[kTileKeys];
+                if (live) key_range(a.shape, u.q, u.u.row0 + in, u.u.row0 + in + 1, lo, hi);
+                const uint32_t unit_key0 = (u.u.tile0 + u.tile0) * kTileKeys;
+                for (uint32_t j = 0; ok && j < tiles; ++j, next_tile()) {
+                    if ((n & 1) != g) continue;
+                    if (!(ok = __all_sync(0xffffffffu, bar_wait(bar(B_S + n6), n6_phase, &dead)))) break;
+                    bool heard = j < 2;  // of the reference after the tile before
+                    if (j == 1) {
+                        if (!(ok = __all_sync(0xffffffffu, settled(n - 1)))) break;
+                        ref = refs[row];
+                    }
+                    if (live_rows) {
+                        fence_after();
+                        const uint32_t key0 = unit_key0 + j * kTileKeys, src = tmem + G::S + nb * kTileKeys + lanes;
+                        const bool whole = __all_sync(0xffffffffu, (key0 >= lo && key0 + kTileKeys <= hi) || !live);
+                        auto hide = [&](float(&s)[32], uint32_t k0) {  // scores of keys that this row does not see
+                            auto below = [&](uint32_t end) {  // bits of the keys before `end`
+                                const uint32_t at = key0 + k0;
+                                return end <= at ? 0u : end - at >= 32 ? 0xffffffffu : (1u << (end - at)) - 1u;
+                            };
+                            const uint32_t seen = below(hi) & ~below(lo);
 #pragma unroll
-                        for (uint32_t k = 0; k < kTileKeys; k += 32) tmem_ld32(tmem + buf * kTileKeys + k + lanes, s + k);
-                        tmem_ld_wait();
-                        const uint32_t key0 = (w.u.tile0 + w.tile0 + j) * kTileKeys;
-                        if (__any_sync(0xffffffffu, key0 < lo || key0 + kTileKeys > hi)) {
+                            for (uint32_t k = 0; k < 32; ++k)
+                                if (!(seen >> k & 1)) s[k] = -INFINITY;
+                        };
+                        uint32_t p[kTileKeys / 2];
+                        f32x2 tile_sum;
+                        // Weights against the reference, packed into p, and their sum. A quarter at a time, the next one on its way.
+                        auto weigh = [&](auto fast) {
+                            const float m = ref == -INFINITY ? 0.f : ref;
+                            const f32x2 mm = pack2(-m, -m);
+                            f32x2 part[2] = {0, 0};
+                            float s[2][32];
+                            tmem_ld32(src, s[0]);
 #pragma unroll
-                            for (uint32_t k = 0; k < kTileKeys; ++k)
-                                if (key0 + k < lo || key0 + k >= hi) s[k] = -INFINITY;
+                            for (uint32_t k0 = 0; k0 < kTileKeys; k0 += 32) {
+                                float(&now)[32] = s[k0 / 32 & 1];
+                                tmem_ld_wait();
+                                if (k0 + 32 < kTileKeys) tmem_ld32(src + k0 + 32, s[k0 / 32 + 1 & 1]);
+                                if constexpr (!decltype(fast)::value) {
+                                    if (!whole) hide(now, k0);
+                                }
+#pragma unroll
+                                for (uint32_t k = 0; k < 32; k += 2) {
+                                    const f32x2 v = fma2(pack2(now[k], now[k + 1]), cc, mm);
+                                    float x, y;
+                                    if (decltype(fast)::value && k % 8 == 6) {
+                                        exp2_pair<T>(v, x, y);
+                                    } else {
+                                        unpack2(v, x, y);
+                                        x = ex2(x);
+                                        y = ex2(y);
+                                    }
+                                    part[k / 2 & 1] = fma2(pack2(x, y), one, part[k / 2 & 1]);
+                                    p[(k0 + k) / 2] = pack_pair<T>(x, y);
+                                }
+                                keep16(p + k0 / 2, part);
+                            }
+                            tile_sum = fma2(part[0], one, part[1]);
+                            float x, y;
+                            unpack2(tile_sum, x, y);
+                            return x + y;
+                        };
+                        bool good = false;
+                        if (whole && j > 0) {
+                            // the usual tile: every key is seen, the reference stands. Whether the tile before has raised it is known by
+                            // then, or waited for below.
+                            const float total = weigh(std::true_type());
+                            const bool known = heard || bar_try(bar(B_REF + quarter * 2 + (n - 1 & 1)), n - 1 >> 1 & 1);
+                            good = __all_sync(0xffffffffu, known && (!live || (refs[row] == ref && ref != -INFINITY && total <= Weights<T>::limit)));
                         }
-                        float m4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                        for (uint32_t k = 4; k < kTileKeys; k += 8)
-#pragma unroll
-                            for (uint32_t x = 0; x < 4; ++x)
-                                m4[x] = k + 4 + x < kTileKeys ? fmaxf(fmaxf(m4[x], s[k + x]), s[(k + 4 + x) % kTileKeys]) : fmaxf(m4[x], s[k + x]);
-                        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
-                        const bool grow = mx > ref + 8.f || (ref == -INFINITY && mx > ref);
-                        if (__any_sync(0xffffffffu, grow)) {
-                            const float f = grow ? ex2(ref - mx) : 1.f;  // ref = -inf: 0, and nothing but zeros was added
-                            if (grow) ref = mx;
-                            const f32x2 ff = pack2(f, f);
-                            sums[0] = mul2(sums[0], ff);
-                            sums[1] = mul2(sums[1], ff);
+                        if (!good) {
+                            if (!heard && !(ok = __all_sync(0xffffffffu, settled(n - 1)))) break;
+                            bool raise = live;
                             if (j > 0) {
-                                // The output belongs to the product of the key tile before. With two tiles of rows that one has finished: it was
-                                // issued before the scores that this warp waited for. With one, the scores are a tile ahead of it.
-                                if (!two) {
-                                    const uint32_t before = o ^ 1;
-                                    if (!(ok = __all_sync(0xffffffffu, bar_wait(o_done + before * 8, (done[before] - 1) & 1, &dead)))) break;
-                                    fence_after();
-                                }
+                                const float now = refs[row], f = now == ref ? 1.f : ex2(ref - now);
+                                sums = mul2(sums, pack2(f, f));
+                                ref = now;
+                                const float total = weigh(std::false_type());
+                                raise = live && (!(total <= Weights<T>::limit) || ref == -INFINITY);
+                            }
+                            if (__any_sync(0xffffffffu, raise)) {
+                                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-                                for (uint32_t d = 0; d < D; d += 16) {
-                                    float v[16];
-                                    tmem_ld16(tmem + 256 + t * D + d + lanes, v);
+                                for (uint32_t k0 = 0; k0 < kTileKeys; k0 += 32) {
+                                    float s[32];
+                                    tmem_ld32(src + k0, s);
                                     tmem_ld_wait();
+                                    if (!whole) hide(s, k0);
 #pragma unroll
-                                    for (int i = 0; i < 16; ++i) v[i] *= f;
-                                    tmem_st16(tmem + 256 + t * D + d + lanes, v);
+                                    for (uint32_t k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], s[k]);
                                 }
+                                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
+                                const float now = raise ? fmaxf(ref, mx) : ref;
+                                if (j > 0 && __any_sync(0xffffffffu, now != ref)) {
+                                    const float f = now == ref ? 1.f : ex2(ref - now);  // ref = -inf: 0, and nothing but zeros was added
+                                    sums = mul2(sums, pack2(f, f));
+                                    // the output belongs to the product of the tile before until that has finished, and the next one waits for this warp
+                                    if (!(ok = __all_sync(0xffffffffu, bar_wait(bar(B_PV + (n - 1 & 1)), n - 1 >> 1 & 1, &dead)))) break;
+                                    fence_after();
+#pragma unroll 1
+                                    for (uint32_t d = 0; d < D; d += 16) {
+                                        float v[16];
+                                        tmem_ld16(tmem + G::O + d + lanes, v);
+                                        tmem_ld_wait();
+#pragma unroll
+                                        for (int i = 0; i < 16; ++i) v[i] *= f;
+                                        tmem_st16(tmem + G::O + d + lanes, v);
+                                    }
+                                }
+                                ref = now;
+                                refs[row] = ref;
+                                if (j == 0) {  // the other group may begin with the next tile
+                                    __syncwarp();
+                                    if (lane == 0) bar_arrive(bar(B_REF + quarter * 2 + (n & 1)));
+                                }
+                                weigh(std::false_type());
                             }
                         }
-                        const float m = ref == -INFINITY ? 0.f : ref;
-                        const f32x2 cc = pack2(c, c), mm = pack2(-m, -m), one = pack2(1.f, 1.f);
-#pragma unroll
-                        for (uint32_t k0 = 0; k0 < kTileKeys; k0 += 32) {
-                            uint32_t p[16];
-#pragma unroll
-                            for (uint32_t k = 0; k < 32; k += 2) {
-                                float x, y;
-                                unpack2(fma2(pack2(s[k0 + k], s[k0 + k + 1]), cc, mm), x, y);
-                                x = ex2(x);
-                                y = ex2(y);
-                                sums[k / 2 & 1] = fma2(pack2(x, y), one, sums[k / 2 & 1]);
-                                p[k / 2] = pack_pair<T>(x, y);
-                            }
-                            tmem_st16(tmem + buf * kTileKeys + k0 / 2 + lanes, reinterpret_cast<const float *>(p));
+                        if (!ok) break;
+                        sums = fma2(tile_sum, one, sums);
+                        if (j > 0) {
+                            __syncwarp();
+                            if (lane == 0) bar_arrive(bar(B_REF + quarter * 2 + (n & 1)));
                         }
+                        tmem_st32(src, p);
+                        tmem_st32(src + 32, p + 32);
                         tmem_st_wait();
                         fence_before();
+                    } else {
+                        if (!heard && !(ok = __all_sync(0xffffffffu, settled(n - 1)))) break;
+                        if (lane == 0) bar_arrive(bar(B_REF + quarter * 2 + (n & 1)));
                     }
-                    if (!two) ++done[o];
                     __syncwarp();
-                    if (lane == 0) bar_arrive(p_full + b * 8);
+                    if (lane == 0) bar_turn_leader(leader_addr(bar(B_P + n6)));
                 }
                 if (!ok) break;
-                if (!(ok = __all_sync(0xffffffffu, bar_wait(fin + t * 8, units & 1, &dead)))) break;
-                ++units;
+                // the unit's products, the last reference, and the other group's sums
+                ok = bar_wait(bar(B_END), units & 1, &dead) && settled(n - 1);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
                 fence_after();
+                const float now = refs[row];
+                if (now != ref) {
+                    const float f = ex2(ref - now);
+                    sums = mul2(sums, pack2(f, f));
+                    ref = now;
+                }
             }
-            if (t > 0 && !two) continue;
-            float sum, x[4];
-            unpack2(sums[0], x[0], x[1]);
-            unpack2(sums[1], x[2], x[3]);
-            sum = (x[0] + x[1]) + (x[2] + x[3]);
-            if (w.begins && w.ends) {
+            float x, y;
+            unpack2(sums, x, y);
+            float sum = x + y;
+            if (tiles) {
+                sums_of[g][row] = sum;
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar(B_SUM + quarter));
+                if (!(ok = __all_sync(0xffffffffu, bar_wait(bar(B_SUM + quarter), units & 1, &dead)))) break;
+                ++units;
+                sum = sums_of[0][row] + sums_of[1][row];
+            }
+            const uint32_t o = tmem + G::O + g * (D / 2) + lanes;  // this group's half of the dimensions
+            if (whole_unit) {
                 float inv = 0.f;
-                if (sum != 0.f) {
-                    if (a.op.sinks && live) sum += ex2(fmaf(a.op.sinks[head], 1.4426950408889634f, -ref));
+                if (sum != 0.f && live) {
+                    if (a.op.sinks) sum += ex2(fmaf(a.op.sinks[u.at.head * a.shape.group + (u.u.row0 + in) % a.shape.group], 1.4426950408889634f, -ref));
                     inv = 1.0f / sum;
                 }
-                T *out = (T *)a.op.out + (uint64_t)token * a.op.out_token_stride + (uint64_t)head * a.op.out_head_stride;
+                // through shared memory, where the queries were
+                const bool none = sum == 0.f;
 #pragma unroll 1
-                for (uint32_t d = 0; d < D; d += 32) {
+                for (uint32_t d = 0; d < D / 2; d += 32) {
                     float v[32];
-                    tmem_ld32(tmem + 256 + t * D + d + lanes, v);
-                    tmem_ld_wait();
-                    if (live) {
+                    if (tiles) {
+                        tmem_ld32(o + d, v);
+                        tmem_ld_wait();
+                    }
 #pragma unroll
-                        for (uint32_t i = 0; i < 32; i += 8)
-                            *reinterpret_cast<uint4 *>(out + d + i) =
-                                sum == 0.f ? make_uint4(0, 0, 0, 0)
-                                           : make_uint4(pack_pair<T>(v[i] * inv, v[i + 1] * inv), pack_pair<T>(v[i + 2] * inv, v[i + 3] * inv),
-                                                        pack_pair<T>(v[i + 4] * inv, v[i + 5] * inv), pack_pair<T>(v[i + 6] * inv, v[i + 7] * inv));
+                    for (uint32_t i = 0; i < 32; i += 8) {
+                        const uint32_t col = g * P + (d + i) / 8;
+                        uint4 h = make_uint4(pack_pair<T>(v[i] * inv, v[i + 1] * inv), pack_pair<T>(v[i + 2] * inv, v[i + 3] * inv),
+                                             pack_pair<T>(v[i + 4] * inv, v[i + 5] * inv), pack_pair<T>(v[i + 6] * inv, v[i + 7] * inv));
+                        if (none) h = make_uint4(0, 0, 0, 0);
+                        store16(here + (col >> 3) * (kTileRows * 128) + row * 128 + (((col & 7) ^ (row & 7)) << 4), h);
                     }
                 }
+                __syncwarp();
+                const unsigned long long out = row_of(a.op.out, a.op.out_token_stride, a.op.out_head_stride);
+#pragma unroll 4
+                for (uint32_t i = 0; i < P; ++i) {
+                    uint32_t from;
+                    const uint32_t d = piece_of(i, from);
+                    T *dst = (T *)__shfl_sync(0xffffffffu, out, from);
+                    if (live_rows >> from & 1) reinterpret_cast<uint4 *>(dst)[lane % P] = load16(d);
+                }
+                __syncwarp();
             } else {
-                const uint32_t BR = G::NQ * kTileRows;
-                float *slot = a.partial + (blockIdx.x * 2ull + (w.begins ? 1 : 0)) * slot_floats(BR, D);
-                slot[in] = ref;
-                slot[BR + in] = sum;
-                float4 *part = reinterpret_cast<float4 *>(slot + 2 * BR);
-                if (tiles)
+                constexpr uint32_t BR = 2 * kTileRows;
+                float *slot = a.partial + (piece * 2ull + (u.begins ? 1 : 0)) * slot_floats(BR, D);
+                if (g == 0) {
+                    slot[in] = ref;
+                    slot[BR + in] = sum;
+                }
+                float4 *part = reinterpret_cast<float4 *>(slot + 2 * BR) + (uint64_t)g * (D / 8) * BR + in;
+                if (tiles && live_rows)
 #pragma unroll 1
-                    for (uint32_t d = 0; d < D; d += 16) {
+                    for (uint32_t d = 0; d < D / 2; d += 16) {
                         float v[16];
-                        tmem_ld16(tmem + 256 + t * D + d + lanes, v);
+                        tmem_ld16(o + d, v);
                         tmem_ld_wait();
 #pragma unroll
-                        for (uint32_t i = 0; i < 16; i += 4) part[((d + i) / 4) * BR + in] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        for (uint32_t i = 0; i < 16; i += 4) part[(d + i) / 4 * BR] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                     }
             }
             fence_before();  // the next unit's products write the output
         }
-        if (!shares && tid == 0) a.shared[blockIdx.x].sharers = 0;
+        if (!shares && tid == 0 && rank == 0) a.shared[piece].sharers = 0;
     }
+    if (!ok && lane == 0) *error_word = DEV_ERR_WAIT_TIMEOUT;
     __syncwarp();
+    fence_before();
     __syncthreads();
+    cluster_sync();  // the other CTA's last arrivals here and products in this CTA's memory
     if (warp == kIssueWarp) {
         fence_after();
-        tmem_free(tmem, 512);
+        tmem_free_pair(tmem, 512);
     }
-    if (tid == 0 && dead) *error_word = DEV_ERR_WAIT_TIMEOUT;
 }
 
 template <typename T, int D>
 ctox_status tile_launch(ctox_ctx *ctx, AttnArgs &a) {
     using G = Tile<D>;
-    a.box = kTileKeys;
+    a.box = kTileKeys / 2;
     while (a.op.kv.page_tokens % a.box) a.box /= 2;
     CUtensorMap mk, mv;
-    EX(cache_map(ctx, &mk, a.op, a.op.kv.k, a.box, G::CH));
-    EX(cache_map(ctx, &mv, a.op, a.op.kv.v, a.box, G::CH));
-    const size_t room = (size_t)ctx->max_smem_optin - 1024;  // static shared memory
+    EX(cache_map(ctx, &mk, a.op, a.op.kv.k, a.box, D / 64));
+    EX(cache_map(ctx, &mv, a.op, a.op.kv.v, a.box, G::VC, G::VW));
+    const size_t room = (size_t)ctx->max_smem_optin - 4096;  // static shared memory
     const uint32_t slots = G::slots(room, a.op.n_requests);
     const size_t smem = G::smem(slots, a.op.n_requests);
     auto kernel = k_attention_tile<T, D>;
     CTOX_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    CTOX_CUDA(ctx, launch_pdl(kernel, dim3((uint32_t)ctx->sm_count), dim3(kTileThreads), smem, ctx->stream, mk, mv, a, slots, ctx->dev_error));
+    CTOX_CUDA(ctx, launch_pdl_cluster(kernel, dim3((uint32_t)ctx->sm_count / 2 * 2), dim3(kTileThreads), smem, ctx->stream, 2, mk, mv, a, slots,
+                                      ctx->dev_error));
     return CTOX_OK;
 }
 template <typename T>
@@ -437,12 +700,10 @@ ctox_status tile_launch(ctox_ctx *ctx, AttnArgs &a) {
 
 }  // namespace
 
-uint32_t tile_block_rows(uint32_t dim) { return dim == 256 ? kTileRows : 2 * kTileRows; }
-
 ctox_status launch_attention_tile(ctox_ctx *ctx, AttnArgs &a) {
-    a.shape.block_rows = tile_block_rows(a.op.dim);
-    a.shape.half_rows = kTileRows;
-    a.shape.key_tile = kTileKeys;
+    a.shape.block_rows = kTileBlockRows;
+    a.shape.half_rows = kTileBlockRows;  // a pair's products take as long with fewer rows
+    a.shape.key_shift = 7;
     return a.op.kv.dtype == CTOX_BF16 ? tile_launch<__nv_bfloat16>(ctx, a) : tile_launch<__half>(ctx, a);
 }
 

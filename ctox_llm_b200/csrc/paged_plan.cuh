@@ -24,7 +24,7 @@ struct Request {
 
 struct Shape {
     uint32_t kv_heads, group;        // query heads per KV head
-    uint32_t block_rows, key_tile;   // of a unit, of a key tile
+    uint32_t block_rows, key_shift;  // of a unit; log2 of a key tile
     uint32_t half_rows;              // up to that many rows in a block a tile costs 1, else 2
     uint32_t overhead;               // of a unit, in tiles
     uint32_t least_rows, most_rows;  // requests with other numbers of rows (tokens x group) are not this kernel's
@@ -61,27 +61,42 @@ CTOX_HD Unit unit_of(const Shape &s, const Request &q, uint32_t block) {
     u.row0 = block * s.block_rows;
     u.rows = rows - u.row0 < s.block_rows ? rows - u.row0 : s.block_rows;
     key_range(s, q, u.row0, u.row0 + u.rows, u.lo, u.hi);
-    u.tile0 = u.lo / s.key_tile;
-    u.tiles = u.hi > u.lo ? (u.hi + s.key_tile - 1) / s.key_tile - u.tile0 : 0;
+    u.tile0 = u.lo >> s.key_shift;
+    u.tiles = u.hi > u.lo ? ((u.hi - 1) >> s.key_shift) + 1 - u.tile0 : 0;
     u.weight = u.rows > s.half_rows ? 2 : 1;
     u.cost = s.overhead + u.tiles * u.weight;
     return u;
 }
 
-// Cuts. `total` is the line's length, `ctas` the most pieces; pieces shorter than `least` are not worth a CTA.
-CTOX_HD uint32_t pieces_of(uint64_t total, uint32_t ctas, uint32_t least) {
-    const uint64_t n = total / least;
-    return n < 1 ? 1 : n < ctas ? (uint32_t)n : ctas;
+// Where the line is cut: into equal pieces, one per CTA, but none shorter than `least`, which is not worth a CTA.
+struct Cuts {
+    uint64_t total, each;
+    uint32_t pieces, rest, least;
+};
+CTOX_HD Cuts cuts_of(uint64_t total, uint32_t ctas, uint32_t least) {
+    Cuts c;
+    c.total = total;
+    c.least = least;
+    c.pieces = total >= (uint64_t)least * ctas ? ctas : (uint32_t)total / least;
+    if (!c.pieces && total) c.pieces = 1;
+    c.each = c.pieces ? total / c.pieces : 0;
+    c.rest = (uint32_t)(total - c.each * c.pieces);
+    return c;
 }
-CTOX_HD uint64_t raw_cut(uint64_t total, uint32_t pieces, uint32_t i) { return total * i / pieces; }
+CTOX_HD uint64_t raw_cut(const Cuts &c, uint32_t i) { return c.each * i + c.rest * i / c.pieces; }  // rest, i <= pieces: 32 bits
 // A unit this short is not cut.
 CTOX_HD bool keeps_whole(uint32_t cost, uint32_t least) { return cost < 2 * least; }
-CTOX_HD uint64_t cut_in_unit(uint64_t x, uint64_t start, uint32_t cost, uint32_t least) {
-    return !keeps_whole(cost, least) ? x : 2 * (x - start) <= cost ? start : start + cost;
-}
 // CTAs that share a unit which starts in piece `first` and ends at `end`.
-CTOX_HD uint32_t sharers(uint64_t total, uint32_t pieces, uint32_t first, uint64_t end) {
-    return (uint32_t)((end * pieces + total - 1) / total - 1 - first) + 1;
+CTOX_HD uint32_t sharers(const Cuts &c, uint32_t first, uint64_t end) {
+    uint32_t lo = first, hi = c.pieces;  // the last cut before `end` is in [lo, hi)
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (raw_cut(c, mid) < end)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo - first + 1;
 }
 // Tiles of a unit before place x of the line.
 CTOX_HD uint32_t tiles_before(const Shape &s, const Unit &u, uint64_t start, uint64_t x) {
@@ -91,7 +106,8 @@ CTOX_HD uint32_t tiles_before(const Shape &s, const Unit &u, uint64_t start, uin
     return t < u.tiles ? t : u.tiles;
 }
 
-// A place on the line and the unit there. Line: n requests, at(i) their places (at(n) the end), request(i, q) their numbers.
+// A place on the line and the unit there. Line: n requests, at(i) their places (at(n) the end), per_head(i) a KV head's share,
+// request(i, q) their numbers.
 struct Cut {
     uint64_t x, start;  // start: of the unit
     uint32_t request, head, block;
@@ -148,25 +164,32 @@ CTOX_HD Cut locate(const Shape &s, const Line &line, uint64_t x) {
     c.request = lo;
     Request q;
     line.request(lo, q);
-    const uint64_t per_head = (line.at(lo + 1) - line.at(lo)) / s.kv_heads, in = x - line.at(lo);
-    c.head = (uint32_t)(in / per_head);
+    const uint64_t per_head = line.per_head(lo), in = x - line.at(lo);
+    c.head = (uint32_t)((float)in / (float)per_head);  // one off at most, for the rounding
+    if (c.head >= s.kv_heads) c.head = s.kv_heads - 1;
+    while (c.head * per_head > in) --c.head;
+    while ((c.head + 1) * per_head <= in) ++c.head;
     uint64_t off = in - c.head * per_head;
     c.block = find_block(s, q, off);
     c.start = line.at(lo) + c.head * per_head + off;
     return c;
 }
-// Cut i of `pieces`, moved out of a unit that is too short to be cut.
+// Cut i, moved to the nearer end of a unit that is too short to be cut.
 template <class Line>
-CTOX_HD Cut cut_at(const Shape &s, const Line &line, uint64_t total, uint32_t pieces, uint32_t i, uint32_t least) {
-    const uint64_t x = raw_cut(total, pieces, i);
-    if (x >= total) return Cut{total, total, 0, 0, 0};
+CTOX_HD Cut cut_at(const Shape &s, const Line &line, const Cuts &cuts, uint32_t i) {
+    const uint64_t x = i < cuts.pieces ? raw_cut(cuts, i) : cuts.total;
+    if (x >= cuts.total) return Cut{cuts.total, cuts.total, 0, 0, 0};
     Cut c = locate(s, line, x);
     Request q;
     line.request(c.request, q);
     const uint32_t cost = unit_of(s, q, c.block).cost;
-    c.x = cut_in_unit(x, c.start, cost, least);
-    if (c.x < c.start + cost) return c;
-    return c.x >= total ? Cut{total, total, 0, 0, 0} : locate(s, line, c.x);
+    if (!keeps_whole(cost, cuts.least)) return c;
+    if (2 * (x - c.start) <= cost) {
+        c.x = c.start;
+        return c;
+    }
+    const uint64_t next = c.start + cost;
+    return next >= cuts.total ? Cut{cuts.total, cuts.total, 0, 0, 0} : locate(s, line, next);
 }
 
 // A CTA's share of the line, unit by unit.

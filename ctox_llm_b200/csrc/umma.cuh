@@ -162,6 +162,14 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b,
         "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
+// A in tensor memory: each CTA its own 128 rows, at the same columns.
+__device__ __forceinline__ void mma_f16_ts_pair(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
 // D = A B + D / 2^SHIFT, by one CTA or a pair.
 template <uint32_t G, uint32_t SHIFT>
 __device__ __forceinline__ void mma_f16_shifted(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {

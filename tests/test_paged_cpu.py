@@ -122,7 +122,9 @@ WALK = r"""
 using namespace ctox::paged;
 struct HostLine {
     const Request *q; const uint64_t *places; uint32_t n;
+    uint32_t kv_heads;
     uint64_t at(uint32_t i) const { return places[i]; }
+    uint64_t per_head(uint32_t i) const { return (places[i + 1] - places[i]) / kv_heads; }
     void request(uint32_t i, Request &r) const { r = q[i]; }
 };
 // rows out: cta, request, head, block, first tile of the unit, tile0, tile1, begins, ends, sharers (where it begins and goes on)
@@ -133,19 +135,17 @@ extern "C" long deal(const Shape *s, const Request *q, uint32_t n, uint32_t ctas
         for (uint32_t b = 0; b < blocks_of(*s, q[i]); ++b) cost += unit_of(*s, q[i], b).cost;
         at[i + 1] = at[i] + cost * s->kv_heads;
     }
-    const HostLine line{q, at.data(), n};
-    const uint64_t total = at[n];
-    if (!total) return 0;
-    const uint32_t pieces = pieces_of(total, ctas, least);
+    const HostLine line{q, at.data(), n, s->kv_heads};
+    const Cuts cuts = cuts_of(at[n], ctas, least);
     long k = 0;
-    for (uint32_t c = 0; c < pieces; ++c) {
+    for (uint32_t c = 0; c < cuts.pieces; ++c) {
         Walk w;
-        w.at = cut_at(*s, line, total, pieces, c, least);
-        w.end = cut_at(*s, line, total, pieces, c + 1, least).x;
+        w.at = cut_at(*s, line, cuts, c);
+        w.end = cut_at(*s, line, cuts, c + 1).x;
         for (; walk_unit(*s, line, w); walk_on(*s, line, w)) {
             if (k >= room) return -1;
             const uint32_t r[10] = {c, w.at.request, w.at.head, w.at.block, w.u.tile0, w.tile0, w.tile1, w.begins, w.ends,
-                                    w.begins && !w.ends ? sharers(total, pieces, c, w.at.start + w.u.cost) : 0};
+                                    w.begins && !w.ends ? sharers(cuts, c, w.at.start + w.u.cost) : 0};
             for (uint32_t j = 0; j < 10; ++j) out[k * 10 + j] = r[j];
             ++k;
         }
@@ -165,7 +165,8 @@ def deal(tmp_path_factory):
     lib.deal.restype = C.c_long
 
     def run(shape, requests, ctas, least):
-        s = np.array([shape[k] for k in ("kv_heads", "group", "block_rows", "key_tile", "half_rows", "overhead", "least_rows", "most_rows",
+        shape = dict(shape, key_shift=shape["key_tile"].bit_length() - 1)
+        s = np.array([shape[k] for k in ("kv_heads", "group", "block_rows", "key_shift", "half_rows", "overhead", "least_rows", "most_rows",
                                          "causal", "window")], dtype=np.uint32)
         q = np.array(requests, dtype=np.uint32).reshape(-1, 3)
         out = np.zeros((400000, 10), dtype=np.uint32)
