@@ -32,15 +32,16 @@ struct Tile {
     static constexpr uint32_t NB = D == 256 ? 2 : 3;            // score buffers: what tensor memory holds beside the output
     static constexpr uint32_t SLOT = 128 * D;                   // of the ring: 64 keys, or half the dimensions of 128 values
     static constexpr uint32_t Q_BYTES = kTileRows * D * 2;
+    static constexpr uint32_t QB = D == 256 ? 1 : 2;            // buffers of queries: the next unit's beside this one's, if there is room
     static constexpr uint32_t VW = D == 64 ? 32 : 64;           // dimensions in a swizzled row of a value tile
     static constexpr uint32_t VC = D / 2 / VW;                  // chunks of them in this CTA's half
     static constexpr uint32_t V_GROUP = 8 * VW * 2 * VC;        // bytes of eight values
     static constexpr uint32_t O = 0, S = D == 256 ? 256 : 128;  // columns of tensor memory
     static uint32_t slots(size_t room, uint32_t n) {
-        const uint32_t s = (uint32_t)((room - 1024 - Q_BYTES - (n + 1) * 8) / SLOT);
+        const uint32_t s = (uint32_t)((room - 1024 - QB * Q_BYTES - (n + 1) * 8) / SLOT);
         return s < kMostSlots ? s : kMostSlots;
     }
-    static size_t smem(uint32_t slots, uint32_t n) { return 1024 + Q_BYTES + (size_t)slots * SLOT + (n + 1) * 8; }
+    static size_t smem(uint32_t slots, uint32_t n) { return 1024 + QB * Q_BYTES + (size_t)slots * SLOT + (n + 1) * 8; }
 };
 
 template <typename T>
@@ -130,7 +131,8 @@ enum : uint32_t {
     B_P = B_S + 6,                     // [6] at the first CTA: weights, by four warps of each
     B_REF = B_P + 6,                   // [4 quarters][2]: the reference is settled for tile n, by its warp
     B_SUM = B_REF + 8,                 // [4 quarters]: both groups' sums
-    B_PV = B_SUM + 4,                  // [2] both CTAs: output of tile n
+    B_OUT = B_SUM + 4,                 // [4 quarters]: both groups have read the output
+    B_PV = B_OUT + 4,                  // [2] both CTAs: output of tile n
     B_Q = B_PV + 2,                    // at the first CTA: queries, by eight warps of each
     B_END = B_Q + 1,                   // both CTAs: the unit's products
     B_DRAINED = B_END + 1,
@@ -146,13 +148,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     extern __shared__ uint8_t raw[];
     __shared__ __align__(8) uint64_t bars[B_COUNT];
     __shared__ unsigned long long scan[32];
-    __shared__ float refs[kTileRows], sums_of[2][kTileRows];
+    __shared__ float refs[kTileRows], sums_of[2][2][kTileRows];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
     __shared__ Cut cuts[2];
-    __shared__ Walk walks[8];
+    __shared__ Walk walks[8][2];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster_rank(), piece = blockIdx.x >> 1;
-    const uint32_t base = (smem_addr(raw) + 1023) & ~1023u, q_s = base, ring = q_s + G::Q_BYTES;
+    const uint32_t base = (smem_addr(raw) + 1023) & ~1023u, q_s = base, ring = q_s + G::QB * G::Q_BYTES;
     unsigned long long *at = reinterpret_cast<unsigned long long *>(raw + (ring + slots * G::SLOT - smem_addr(raw)));
     const uint32_t b0 = smem_addr(bars);
     auto bar = [&](uint32_t i) { return b0 + i * 8; };
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             bar_init(bar(B_P + i), 8);
         }
         for (uint32_t i = 0; i < 8; ++i) bar_init(bar(B_REF + i), 1);
-        for (uint32_t i = 0; i < 4; ++i) bar_init(bar(B_SUM + i), 2);
+        for (uint32_t i = 0; i < 8; ++i) bar_init(bar(B_SUM + i), 2);  // and B_OUT
         bar_init(bar(B_PV), 1);
         bar_init(bar(B_PV + 1), 1);
         bar_init(bar(B_Q), 16);
@@ -214,14 +216,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
                 const int32_t *table = table_row(a, w.at.request);
                 const uint32_t tiles = w.tile1 - w.tile0, first = (w.u.tile0 + w.tile0) * kTileKeys + lane * a.box;
-                // Order of the ring: the keys of as many tiles as there are score buffers, then values and keys in turn. `entry`: this lane's page
-                // of a tile, INT32_MIN where no row sees what its box holds. Entries of the table are read one tile ahead.
-                auto entry = [&](uint32_t j) {
-                    const uint32_t token = first + j * kTileKeys;
-                    return j < tiles && lane < boxes && token < w.u.hi && token + a.box > w.u.lo ? table[page_index(a, token)] : INT32_MIN;
+                // Order of the ring: the keys of as many tiles as there are score buffers, then values and keys in turn. A warp holds the table's entries
+                // of four tiles, eight lanes for a tile's boxes (INT32_MIN: no row sees what the box holds), and the next four are on their way:
+                // read tile by tile they would hold up every copy.
+                auto entries = [&](uint32_t group) {
+                    const uint32_t j = group * 4 + lane / 8, token = (w.u.tile0 + w.tile0 + j) * kTileKeys + lane % 8 * a.box;
+                    return j < tiles && lane % 8 < boxes && token < w.u.hi && token + a.box > w.u.lo ? table[page_index(a, token)] : INT32_MIN;
                 };
-                auto load = [&](bool keys, uint32_t j, int32_t page) {
-                    const bool mine = page != INT32_MIN && is_page(a, page, error_word);
+                int32_t four = entries(0), next_four = entries(1);
+                uint32_t group4 = 0;
+                auto load = [&](bool keys, uint32_t j) {
+                    const int32_t page = __shfl_sync(0xffffffffu, j / 4 == group4 ? four : next_four, j % 4 * 8 + lane % 8);
+                    const bool mine = lane < 8 && page != INT32_MIN && is_page(a, page, error_word);
                     const uint32_t copies = __popc(__ballot_sync(0xffffffffu, mine)), token = first + j * kTileKeys;
                     const int group = (int)((token - page_index(a, token) * a.op.kv.page_tokens) / 8);
                     const bool edge = !keys && is_edge(j);
@@ -252,19 +258,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         ++round;
                     }
                 };
-                // pages of the tile whose values are next and of those behind it
-                int32_t page[G::NB + 1];
-#pragma unroll
-                for (uint32_t i = 0; i <= G::NB; ++i) page[i] = entry(i);
-#pragma unroll
-                for (uint32_t i = 0; i < G::NB; ++i)
-                    if (ok && i < tiles) load(true, i, page[i]);
+                for (uint32_t k = 0; ok && k < G::NB && k < tiles; ++k) load(true, k);
                 for (uint32_t v = 0; ok && v < tiles; ++v) {
-                    load(false, v, page[0]);
-                    if (ok && v + G::NB < tiles) load(true, v + G::NB, page[G::NB]);
-#pragma unroll
-                    for (uint32_t i = 0; i < G::NB; ++i) page[i] = page[i + 1];
-                    page[G::NB] = entry(v + 1 + G::NB);
+                    if (v / 4 != group4) {  // keys are at most three tiles ahead: in this group or the next
+                        four = next_four;
+                        next_four = entries(++group4 + 1);
+                    }
+                    load(false, v);
+                    if (ok && v + G::NB < tiles) load(true, v + G::NB);
                 }
             }
             if (!ok) {  // leave no copy in flight behind; the barriers may lack the other CTA's part, so by time
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             constexpr uint32_t idesc_s = Weights<T>::idesc(kTileKeys, false), idesc_o = Weights<T>::idesc(D, true);
             const bool issuer = elect_one();
             uint32_t next = 0, next_phase = 0, cleared = 0;  // of the ring; phases of B_CLEAR
-            uint32_t units = 0, s6 = 0, p6 = 0, p6_phase = 0, buffer_s = 0, buffer_p = 0, pv = 0;
+            uint32_t units = 0, q_now = q_s, s6 = 0, p6 = 0, p6_phase = 0, buffer_s = 0, buffer_p = 0, pv = 0;
             auto take = [&](bool edge) {  // the next slot, once it is full
                 const uint32_t slot = next;
                 ok = ok && __all_sync(0xffffffffu, bar_wait(bar(B_FULL + slot), next_phase, &dead));
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             };
             auto scores = [&](uint32_t slot) {  // S = Q K^T of the next tile
                 if (issuer) {
-                    const uint64_t dq = desc_rows(q_s, 1024), dk = desc_rows(ring + slot * G::SLOT, D * 16);
+                    const uint64_t dq = desc_rows(q_now, 1024), dk = desc_rows(ring + slot * G::SLOT, D * 16);
                     const uint32_t d = tmem + G::S + buffer_s * kTileKeys;
 #pragma unroll
                     for (uint32_t k = 0; k < D / 16; ++k)
@@ -308,6 +309,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
                 const uint32_t tiles = w.tile1 - w.tile0;
                 if (!tiles) continue;
+                q_now = q_s + units % G::QB * G::Q_BYTES;
                 if (!(ok = __all_sync(0xffffffffu, bar_wait<BAR_PAIR>(bar(B_Q), units++ & 1, &dead)))) break;
                 for (uint32_t j = 0; ok && j < G::NB && j < tiles; ++j) {
                     const uint32_t slot = take(false);
@@ -388,67 +390,83 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
         };
         auto settled = [&](uint32_t tile) { return bar_wait(bar(B_REF + quarter * 2 + (tile & 1)), tile >> 1 & 1, &dead); };
-        // Where the walk stands is kept in shared memory, one for each warp: in registers it would push scores out of them.
-        Walk &u = walks[warp];
-        if (lane == 0) u = w;
-        for (bool first = true; ok; first = false) {
-            __syncwarp();
-            bool more = true;
-            if (lane == 0) {
-                if (!first) walk_on(a.shape, line, u);
-                more = walk_unit(a.shape, line, u);
+        // Where the walk stands is kept in shared memory, for each warp this unit and the next: in registers it would push scores out of them.
+        // The first turn has no unit yet, only a next one.
+        uint32_t turn = 0;
+        auto at_end = [&](const Walk &u) { return u.q.rows_new == 0xffffffffu; };
+        // the address of this lane's row of q (or out), this group's half of its dimensions
+        auto row_of = [&](const Walk &u, const void *m, uint64_t token_stride, uint64_t head_stride) {
+            const uint32_t r = u.u.row0 + in, t = r / a.shape.group;
+            return (unsigned long long)((const T *)m + (uint64_t)(u.q.q0 + t) * token_stride +
+                                        (uint64_t)(u.at.head * a.shape.group + (r - t * a.shape.group)) * head_stride + g * (D / 2));
+        };
+        // This warp's half (g) of its 32 rows of a buffer of queries: piece i of 16 bytes of this lane, neighbours in a row by neighbouring lanes.
+        auto piece_of = [&](uint32_t buffer, uint32_t i, uint32_t &at_row) {
+            at_row = i * ROWS + lane / P;
+            const uint32_t col = g * P + lane % P, rr = quarter * 32 + at_row;
+            return buffer + (col >> 3) * (kTileRows * 128) + rr * 128 + (((col & 7) ^ (rr & 7)) << 4);
+        };
+        auto buffer_of = [&](uint32_t unit) {
+            uint32_t b = q_s + unit % G::QB * G::Q_BYTES;
+            asm volatile("" : "+r"(b));  // addresses formed where they are used, not kept through the tiles
+            return b;
+        };
+        constexpr uint32_t at_once = P < 8 ? P : 8;
+        auto fetch = [&](const Walk &u, uint32_t i0, uint4(&x)[at_once]) {
+            const unsigned long long q = row_of(u, a.op.q, a.op.q_token_stride, a.op.q_head_stride);
+            const uint32_t live_rows = __ballot_sync(0xffffffffu, in < u.u.rows);
+#pragma unroll
+            for (uint32_t i = 0; i < at_once; ++i) {
+                const uint32_t from = (i0 + i) * ROWS + lane / P;
+                const T *src = (const T *)__shfl_sync(0xffffffffu, q, from);
+                x[i] = live_rows >> from & 1 ? reinterpret_cast<const uint4 *>(src)[lane % P] : make_uint4(0, 0, 0, 0);
             }
-            if (!__shfl_sync(0xffffffffu, more, 0)) break;
+        };
+        auto put = [&](uint32_t buffer, uint32_t i0, const uint4(&x)[at_once]) {
+#pragma unroll
+            for (uint32_t i = 0; i < at_once; ++i) {
+                uint32_t at_row;
+                const uint32_t d = piece_of(buffer, i0 + i, at_row);
+                store16(d, x[i]);
+            }
+        };
+        auto queries_ready = [&]() {
+            proxy_fence();
             __syncwarp();
-            const uint32_t tiles = u.tile1 - u.tile0;
-            const bool whole_unit = u.begins && u.ends;
-            if (u.begins && !u.ends) {
+            if (lane == 0) bar_release_leader(leader_addr(bar(B_Q)));
+        };
+        auto load_queries = [&](const Walk &u, uint32_t unit) {
+            const uint32_t buffer = buffer_of(unit);
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < P; i0 += at_once) {
+                uint4 x[at_once];
+                fetch(u, i0, x);
+                put(buffer, i0, x);
+            }
+            queries_ready();
+        };
+        for (;; ++turn) {
+            const Walk &u = walks[warp][turn & 1 ^ 1];
+            Walk &then = walks[warp][turn & 1];
+            if (turn && at_end(u)) break;
+            if (lane == 0) {
+                then = turn ? u : w;
+                if (turn) walk_on(a.shape, line, then);
+                if (!walk_unit(a.shape, line, then)) then.q.rows_new = 0xffffffffu;
+            }
+            __syncwarp();
+            const uint32_t tiles = turn ? u.tile1 - u.tile0 : 0;
+            const bool whole_unit = turn && u.begins && u.ends;
+            if (turn && u.begins && !u.ends) {
                 shares = true;
                 if (tid == 0 && rank == 0)
                     a.shared[piece] = Shared{sharers(cut, piece, u.at.start + u.u.cost), u.at.request, u.at.head, u.u.row0, u.u.rows};
             }
-            const bool live = in < u.u.rows;
+            const bool live = turn && in < u.u.rows;
             const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
-            // this lane's row of q (or out), this group's half of its dimensions
-            auto row_of = [&](const void *m, uint64_t token_stride, uint64_t head_stride) {
-                const uint32_t r = u.u.row0 + in, t = r / a.shape.group;
-                return (unsigned long long)((const T *)m + (uint64_t)(u.q.q0 + t) * token_stride +
-                                            (uint64_t)(u.at.head * a.shape.group + (r - t * a.shape.group)) * head_stride + g * (D / 2));
-            };
-            // this warp's half (g) of its 32 rows: a piece of 16 bytes per lane, neighbours in a row by neighbouring lanes
-            uint32_t here = q_s;
-            asm volatile("" : "+r"(here));  // addresses formed where they are used, not kept through the tiles
-            auto piece_of = [&](uint32_t i, uint32_t &at_row) {
-                at_row = i * ROWS + lane / P;
-                const uint32_t col = g * P + lane % P, rr = quarter * 32 + at_row;
-                return here + (col >> 3) * (kTileRows * 128) + rr * 128 + (((col & 7) ^ (rr & 7)) << 4);
-            };
             float ref = -INFINITY;
             f32x2 sums = 0;
             if (tiles) {
-                {  // queries; the products of the unit before have finished
-                    const unsigned long long q = row_of(a.op.q, a.op.q_token_stride, a.op.q_head_stride);
-                    constexpr uint32_t at_once = P < 8 ? P : 8;
-#pragma unroll 1
-                    for (uint32_t i0 = 0; i0 < P; i0 += at_once) {
-                        uint4 x[at_once];
-#pragma unroll
-                        for (uint32_t i = 0; i < at_once; ++i) {
-                            const uint32_t from = (i0 + i) * ROWS + lane / P;
-                            const T *src = (const T *)__shfl_sync(0xffffffffu, q, from);
-                            x[i] = live_rows >> from & 1 ? reinterpret_cast<const uint4 *>(src)[lane % P] : make_uint4(0, 0, 0, 0);
-                        }
-#pragma unroll
-                        for (uint32_t i = 0; i < at_once; ++i) {
-                            uint32_t at_row;
-                            const uint32_t d = piece_of(i0 + i, at_row);
-                            store16(d, x[i]);
-                        }
-                    }
-                    proxy_fence();
-                    __syncwarp();
-                    if (lane == 0) bar_release_leader(leader_addr(bar(B_Q)));
-                }
                 uint32_t lo = 0, hi = 0;
                 if (live) key_range(a.shape, u.q, u.u.row0 + in, u.u.row0 + in + 1, lo, hi);
                 const uint32_t unit_key0 = (u.u.tile0 + u.tile0) * kTileKeys;
@@ -583,67 +601,79 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         if (lane == 0) bar_arrive(bar(B_REF + quarter * 2 + (n & 1)));
                     }
                     __syncwarp();
+                    // the first product of a unit writes over the output of the one before
+                    if (j == 0 && units > 0 && !(ok = __all_sync(0xffffffffu, bar_wait(bar(B_OUT + quarter), units - 1 & 1, &dead)))) break;
                     if (lane == 0) bar_turn_leader(leader_addr(bar(B_P + n6)));
                 }
                 if (!ok) break;
+            }
+            // The next unit's queries come while the last products run, if they have a buffer of their own: then its scores are formed while this
+            // unit's output is written.
+            auto next_queries = [&](uint32_t unit) {
+                if (!at_end(then) && then.tile1 > then.tile0) load_queries(then, unit);
+            };
+            if constexpr (G::QB == 2) next_queries(units + (tiles ? 1 : 0));
+            if (tiles) {
                 // the unit's products, the last reference, and the other group's sums
                 ok = bar_wait(bar(B_END), units & 1, &dead) && settled(n - 1);
                 if (!(ok = __all_sync(0xffffffffu, ok))) break;
                 fence_after();
-                const float now = refs[row];
-                if (now != ref) {
-                    const float f = ex2(ref - now);
+                const float last = refs[row];
+                if (last != ref) {
+                    const float f = ex2(ref - last);
                     sums = mul2(sums, pack2(f, f));
-                    ref = now;
+                    ref = last;
                 }
             }
             float x, y;
             unpack2(sums, x, y);
             float sum = x + y;
             if (tiles) {
-                sums_of[g][row] = sum;
+                sums_of[units & 1][g][row] = sum;
                 __syncwarp();
                 if (lane == 0) bar_arrive(bar(B_SUM + quarter));
                 if (!(ok = __all_sync(0xffffffffu, bar_wait(bar(B_SUM + quarter), units & 1, &dead)))) break;
-                ++units;
-                sum = sums_of[0][row] + sums_of[1][row];
+                sum = sums_of[units & 1][0][row] + sums_of[units & 1][1][row];
             }
             const uint32_t o = tmem + G::O + g * (D / 2) + lanes;  // this group's half of the dimensions
-            if (whole_unit) {
+            if (whole_unit && !tiles) {  // no key is seen
+                const unsigned long long out = row_of(u, a.op.out, a.op.out_token_stride, a.op.out_head_stride);
+                if (live)
+                    for (uint32_t i = 0; i < P; ++i) reinterpret_cast<uint4 *>(out)[i] = make_uint4(0, 0, 0, 0);
+            } else if (whole_unit) {
                 float inv = 0.f;
                 if (sum != 0.f && live) {
                     if (a.op.sinks) sum += ex2(fmaf(a.op.sinks[u.at.head * a.shape.group + (u.u.row0 + in) % a.shape.group], 1.4426950408889634f, -ref));
                     inv = 1.0f / sum;
                 }
                 // through shared memory, where the queries were
+                const uint32_t buffer = buffer_of(units);
                 const bool none = sum == 0.f;
 #pragma unroll 1
                 for (uint32_t d = 0; d < D / 2; d += 32) {
                     float v[32];
-                    if (tiles) {
-                        tmem_ld32(o + d, v);
-                        tmem_ld_wait();
-                    }
+                    tmem_ld32(o + d, v);
+                    tmem_ld_wait();
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i += 8) {
                         const uint32_t col = g * P + (d + i) / 8;
                         uint4 h = make_uint4(pack_pair<T>(v[i] * inv, v[i + 1] * inv), pack_pair<T>(v[i + 2] * inv, v[i + 3] * inv),
                                              pack_pair<T>(v[i + 4] * inv, v[i + 5] * inv), pack_pair<T>(v[i + 6] * inv, v[i + 7] * inv));
                         if (none) h = make_uint4(0, 0, 0, 0);
-                        store16(here + (col >> 3) * (kTileRows * 128) + row * 128 + (((col & 7) ^ (row & 7)) << 4), h);
+                        store16(buffer + (col >> 3) * (kTileRows * 128) + row * 128 + (((col & 7) ^ (row & 7)) << 4), h);
                     }
                 }
                 __syncwarp();
-                const unsigned long long out = row_of(a.op.out, a.op.out_token_stride, a.op.out_head_stride);
+                const unsigned long long out = row_of(u, a.op.out, a.op.out_token_stride, a.op.out_head_stride);
 #pragma unroll 4
                 for (uint32_t i = 0; i < P; ++i) {
                     uint32_t from;
-                    const uint32_t d = piece_of(i, from);
+                    const uint32_t d = piece_of(buffer, i, from);
                     T *dst = (T *)__shfl_sync(0xffffffffu, out, from);
                     if (live_rows >> from & 1) reinterpret_cast<uint4 *>(dst)[lane % P] = load16(d);
                 }
                 __syncwarp();
-            } else {
+            } else if (turn) {
                 constexpr uint32_t BR = 2 * kTileRows;
                 float *slot = a.partial + (piece * 2ull + (u.begins ? 1 : 0)) * slot_floats(BR, D);
                 if (g == 0) {
@@ -661,7 +691,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         for (uint32_t i = 0; i < 16; i += 4) part[(d + i) / 4 * BR] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                     }
             }
-            fence_before();  // the next unit's products write the output
+            fence_before();
+            __syncwarp();
+            if (tiles) {
+                if (lane == 0) bar_arrive(bar(B_OUT + quarter));
+                ++units;
+            }
+            if constexpr (G::QB == 1) next_queries(units);
         }
         if (!shares && tid == 0 && rank == 0) a.shared[piece].sharers = 0;
     }
