@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(Rows<D, NT>::NW * 32 + 32)
     __syncthreads();
     pdl_launch();
     pdl_wait();
-    lay_line(a, at, scan, reinterpret_cast<uint32_t *>(aligned), error_word);
+    lay_line(a, at, scan, reinterpret_cast<Listed *>(aligned), error_word);
     const Line line{a, at, a.op.n_requests};
     const Cuts cut = cuts_of(at[a.op.n_requests], gridDim.x, a.least);
     if (blockIdx.x >= cut.pieces) {
@@ -418,7 +418,6 @@ template <typename T, int D, int NT>
 ctox_status rows_launch(ctox_ctx *ctx, AttnArgs &a) {
     using R = Rows<D, NT>;
     a.shape.block_rows = R::BR;
-    a.shape.half_rows = R::BR;
     a.shape.key_shift = R::KT == 64 ? 6 : 7;
     a.box = R::KT;
     while (a.op.kv.page_tokens % a.box) a.box /= 2;
@@ -442,8 +441,8 @@ ctox_status rows_launch(ctox_ctx *ctx, AttnArgs &a) {
 
 }  // namespace
 
-ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attention_op &op, const void *base, uint32_t box, uint32_t chunks,
-                      uint32_t width) {
+ctox_status encode_map(ctox_ctx *ctx, CUtensorMap *map, uint32_t dtype, const void *base, const cuuint64_t (&dims)[5], const cuuint64_t (&strides)[4],
+                       const cuuint32_t (&box)[5], uint32_t swizzle_bytes) {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -456,20 +455,26 @@ ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attentio
         return (Encode)fn;
     }();
     if (!encode) return fail(ctx, CTOX_UNSUPPORTED_OPERATION, "cuTensorMapEncodeTiled is not available");
+    const cuuint32_t each[5] = {1, 1, 1, 1, 1};
+    const CUresult r = encode(map, dtype == CTOX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                              const_cast<void *>(base), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(ctx, CTOX_SHAPE, "paged attention: no tensor map for strides of %llu, %llu, %llu, %llu bytes (error %d)",
+                    (unsigned long long)strides[0], (unsigned long long)strides[1], (unsigned long long)strides[2],
+                    (unsigned long long)strides[3], (int)r);
+    return CTOX_OK;
+}
+ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attention_op &op, const void *base, uint32_t box, uint32_t chunks,
+                      uint32_t width) {
     const ctox_paged_kv &kv = op.kv;
     // one axis runs over pages and heads
     const uint64_t step = op.kv_heads > 1 ? kv.head_stride : kv.page_stride, per_page = op.kv_heads > 1 ? kv.page_stride / kv.head_stride : 1;
     const cuuint64_t dims[5] = {width, 8, op.dim / width, kv.page_tokens / 8, (uint64_t)(kv.n_pages - 1) * per_page + op.kv_heads};
     const cuuint64_t strides[4] = {kv.token_stride * 2, width * 2, kv.token_stride * 16, step * 2};
-    const cuuint32_t boxes[5] = {width, 8, chunks, box / 8, 1}, each[5] = {1, 1, 1, 1, 1};
-    const CUresult r = encode(map, kv.dtype == CTOX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
-                              const_cast<void *>(base), dims, strides, boxes, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-        return fail(ctx, CTOX_SHAPE, "paged attention: a cache of %u pages with strides %llu, %llu, %llu has no tensor map (error %d)", kv.n_pages,
-                    (unsigned long long)kv.page_stride, (unsigned long long)kv.token_stride, (unsigned long long)kv.head_stride, (int)r);
-    return CTOX_OK;
+    const cuuint32_t boxes[5] = {width, 8, chunks, box / 8, 1};
+    return encode_map(ctx, map, kv.dtype, base, dims, strides, boxes, width * 2);
 }
 
 ctox_status launch_attention_rows(ctox_ctx *ctx, AttnArgs &a) {
@@ -527,6 +532,8 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
     if (op->n_tokens && (!op->q || !op->out || !aligned16(op->q) || !aligned16(op->out) || op->q_token_stride % 8 || op->q_head_stride % 8 ||
                          op->out_token_stride % 8 || op->out_head_stride % 8))
         return fail(ctx, CTOX_SHAPE, "%s: q and out want 16-byte aligned matrices and strides of multiples of 8", what);
+    if ((op->n_tokens > 1 && !op->q_token_stride) || (op->heads > 1 && !op->q_head_stride))
+        return fail(ctx, CTOX_SHAPE, "%s: q has one address for several rows", what);
     if (!ctx) return fail(ctx, CTOX_INVALID_STATE, "%s: no context", what);
     if (!op->workspace || !aligned16(op->workspace) || op->workspace_bytes < workspace_bytes(ctx, *op))
         return fail(ctx, CTOX_SHAPE, "%s: workspace of %llu bytes, %llu wanted, aligned to 16", what, (unsigned long long)op->workspace_bytes,
@@ -541,10 +548,8 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
     a.shape.window = op->window;
     a.pages_per_step = op->kv_heads > 1 ? (uint32_t)(op->kv.page_stride / op->kv.head_stride) : 1;
     a.c = op->scale * 1.4426950408889634f;
-    uint32_t bits = 0;
-    while ((1ull << bits) < op->kv.page_tokens) ++bits;
-    a.page_shift = 31 + bits;
-    a.page_factor = (uint32_t)((1ull << a.page_shift) / op->kv.page_tokens + 1);
+    a.by_page = divisor(op->kv.page_tokens);
+    a.shape.by_group = divisor(a.shape.group);
     const DeviceGuard guard(ctx->device);
     CTOX_CUDA(ctx, guard.error());
     // Only the device knows how many rows a request has; the host knows the most, and that a token has `group`.
@@ -552,10 +557,10 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
     const bool many = most > kFewRows, few = !many || (op->n_requests > 1 && a.shape.group <= kFewRows);
     MergePart parts[2] = {};
     uint32_t n_parts = 0;
-    auto merged = [&](uint32_t ctas) {  // where not even the longest unit that there can be is cut, there is nothing to merge
+    auto merged = [&](uint32_t pieces, uint32_t slot_rows) {  // where not even the longest unit that there can be is cut, there is nothing to merge
         const uint64_t longest = a.shape.overhead + ((((uint64_t)op->max_kv_tokens - 1) >> a.shape.key_shift) + 1);
         if (longest <= 0xffffffffu && keeps_whole((uint32_t)longest, a.least)) return;
-        parts[n_parts++] = MergePart{a.shared, a.partial, a.shape.block_rows, ctas};
+        parts[n_parts++] = MergePart{a.shared, a.partial, slot_rows, pieces};
     };
     if (few) {
         a.shape.least_rows = 1;
@@ -565,7 +570,7 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
         a.shared = (Shared *)op->workspace;
         a.partial = (float *)((uint8_t *)op->workspace + descriptor_bytes(ctx));
         EX(launch_attention_rows(ctx, a));
-        merged((uint32_t)ctx->sm_count);
+        merged((uint32_t)ctx->sm_count, a.shape.block_rows);
     }
     if (many) {
         a.shape.least_rows = few ? kFewRows + 1 : 1;
@@ -575,7 +580,7 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
         a.shared = (Shared *)op->workspace + ctx->sm_count;
         a.partial = (float *)((uint8_t *)op->workspace + descriptor_bytes(ctx)) + rows_floats(ctx, op->dim);
         EX(launch_attention_tile(ctx, a));
-        merged((uint32_t)ctx->sm_count / 2);
+        merged((uint32_t)ctx->sm_count / 2, kTileBlockRows);
     }
     if (n_parts) {
         const uint32_t per = 4 * kMergeThreads / op->dim;

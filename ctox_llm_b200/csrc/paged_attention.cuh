@@ -18,7 +18,7 @@ struct AttnArgs {
     Shape shape;
     uint32_t least;          // cost below which a piece of the work is not worth a CTA
     uint32_t box;            // tokens of a copy: what a page and a key tile are both multiples of
-    uint32_t page_factor, page_shift;  // token / page_tokens = token * page_factor >> page_shift, for tokens below 2^31
+    Divisor by_page;         // token / page_tokens
     uint32_t pages_per_step; // page_stride / head_stride where there are several heads, else 1
     float c;                 // scale * log2(e)
     float *partial;          // per CTA two slots: a unit that began before it, one that goes on behind it
@@ -44,9 +44,13 @@ __device__ __forceinline__ const int32_t *table_row(const AttnArgs &a, uint32_t 
 }
 
 // Line places of all requests: at[0 .. n], by the whole block (`scan`: a word per warp). A request's blocks are summed by its thread,
-// but a long prompt's thousands by all threads: such requests are put down in `list` (n words, free to use until the return).
+// but a long prompt's thousands by all threads: such requests are put down in `list` (room for n, free to use until the return).
+struct Listed {
+    Request q;
+    uint32_t index;
+};
 constexpr uint32_t kFewBlocks = 4;
-__device__ __forceinline__ void lay_line(const AttnArgs &a, unsigned long long *at, unsigned long long *scan, uint32_t *list, int32_t *error_word) {
+__device__ __forceinline__ void lay_line(const AttnArgs &a, unsigned long long *at, unsigned long long *scan, Listed *list, int32_t *error_word) {
     __shared__ uint32_t listed;
     const uint32_t n = a.op.n_requests, per = (n + blockDim.x - 1) / blockDim.x, r0 = threadIdx.x * per;
     if (threadIdx.x == 0) listed = 0;
@@ -59,7 +63,7 @@ __device__ __forceinline__ void lay_line(const AttnArgs &a, unsigned long long *
             if (blocks <= kFewBlocks)
                 for (uint32_t b = 0; b < blocks; ++b) cost += unit_of(a.shape, q, b).cost;
             else
-                list[atomicAdd(&listed, 1)] = r;
+                list[atomicAdd(&listed, 1)] = Listed{q, r};
         } else if (blockIdx.x == 0) {
             bad_index(error_word);
         }
@@ -67,12 +71,11 @@ __device__ __forceinline__ void lay_line(const AttnArgs &a, unsigned long long *
     }
     __syncthreads();
     for (uint32_t i = 0, m = listed; i < m; ++i) {
-        Request q;
-        read_request(a, list[i], q);
+        const Request q = list[i].q;
         const uint32_t blocks = blocks_of(a.shape, q);
         unsigned long long cost = 0;
         for (uint32_t b = threadIdx.x; b < blocks; b += blockDim.x) cost += unit_of(a.shape, q, b).cost;
-        if (cost) atomicAdd(&at[list[i] + 1], cost);
+        if (cost) atomicAdd(&at[list[i].index + 1], cost);
     }
     __syncthreads();
     unsigned long long mine = 0;
@@ -98,7 +101,7 @@ struct Line {
 
 // Page of a token for the copies, and its place there.
 __device__ __forceinline__ uint32_t page_index(const AttnArgs &a, uint32_t token) {
-    return (uint32_t)((unsigned long long)token * a.page_factor >> a.page_shift);
+    return divide(token, a.by_page);
 }
 // Whether a table entry is a page; if not, the device error.
 __device__ __forceinline__ bool is_page(const AttnArgs &a, int32_t page, int32_t *error_word) {
@@ -126,6 +129,9 @@ __device__ __forceinline__ int box_step(const AttnArgs &a, int32_t page, uint32_
 }
 #endif
 
+// Five axes, boxes of rows of swizzle_bytes.
+ctox_status encode_map(ctox_ctx *ctx, CUtensorMap *map, uint32_t dtype, const void *base, const cuuint64_t (&dims)[5], const cuuint64_t (&strides)[4],
+                       const cuuint32_t (&box)[5], uint32_t swizzle_bytes);
 // The cache as tensor maps: boxes of `box` tokens by `chunks` * `width` dimensions of one head (width 64, or 32). In shared memory eight
 // tokens are together, 2 * width bytes each, swizzled, chunk after chunk.
 ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attention_op &op, const void *base, uint32_t box, uint32_t chunks,
@@ -134,7 +140,7 @@ ctox_status cache_map(ctox_ctx *ctx, CUtensorMap *map, const ctox_paged_attentio
 // Requests with few rows (paged_attention.cu) and with many (paged_attention_tile.cu).
 ctox_status launch_attention_rows(ctox_ctx *ctx, AttnArgs &a);
 ctox_status launch_attention_tile(ctox_ctx *ctx, AttnArgs &a);
-constexpr uint32_t kTileBlockRows = 256;  // of the latter's units
+constexpr uint32_t kTileBlockRows = 256;  // at most, of the latter's units
 
 }  // namespace paged
 }  // namespace ctox

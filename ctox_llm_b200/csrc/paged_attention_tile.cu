@@ -22,26 +22,26 @@ namespace paged {
 namespace {
 
 constexpr uint32_t kTileRows = 128, kTileKeys = 128, kTileThreads = 384;
-constexpr uint32_t kLoadWarp = 8, kIssueWarp = 9, kClearWarp = 10, kMostSlots = 8;
-// Registers: twelve warps are launched with 168 each. The softmax warps hold a row of 128 scores and take 208; the four others (copies,
-// products, clearing, one without work) keep 88: 8 * 208 + 4 * 88 = 12 * 168.
+constexpr uint32_t kKeyWarp = 8, kIssueWarp = 9, kUnitWarp = 10, kValueWarp = 11, kMostSlots = 4;
+// Registers: twelve warps are launched with 168 each. The softmax warps hold a row of 128 scores and take 208; the four others (copies
+// of keys, products, copies of queries, copies of values) keep 88: 8 * 208 + 4 * 88 = 12 * 168.
 constexpr uint32_t kSoftmaxRegisters = 208, kOtherRegisters = 88;
 
 template <int D>
 struct Tile {
     static constexpr uint32_t NB = D == 256 ? 2 : 3;            // score buffers: what tensor memory holds beside the output
-    static constexpr uint32_t SLOT = 128 * D;                   // of the ring: 64 keys, or half the dimensions of 128 values
+    static constexpr uint32_t SLOT = 128 * D;                   // of the rings: 64 keys, or half the dimensions of 128 values
     static constexpr uint32_t Q_BYTES = kTileRows * D * 2;
     static constexpr uint32_t QB = D == 256 ? 1 : 2;            // buffers of queries: the next unit's beside this one's, if there is room
     static constexpr uint32_t VW = D == 64 ? 32 : 64;           // dimensions in a swizzled row of a value tile
     static constexpr uint32_t VC = D / 2 / VW;                  // chunks of them in this CTA's half
     static constexpr uint32_t V_GROUP = 8 * VW * 2 * VC;        // bytes of eight values
     static constexpr uint32_t O = 0, S = D == 256 ? 256 : 128;  // columns of tensor memory
-    static uint32_t slots(size_t room, uint32_t n) {
-        const uint32_t s = (uint32_t)((room - 1024 - QB * Q_BYTES - (n + 1) * 8) / SLOT);
+    static uint32_t slots(size_t room, uint32_t n) {            // of each ring
+        const uint32_t s = (uint32_t)((room - 1024 - QB * Q_BYTES - (n + 1) * 8) / (2 * SLOT));
         return s < kMostSlots ? s : kMostSlots;
     }
-    static size_t smem(uint32_t slots, uint32_t n) { return 1024 + QB * Q_BYTES + (size_t)slots * SLOT + (n + 1) * 8; }
+    static size_t smem(uint32_t slots, uint32_t n) { return 1024 + QB * Q_BYTES + (size_t)slots * 2 * SLOT + (n + 1) * 8; }
 };
 
 template <typename T>
@@ -123,26 +123,29 @@ __device__ __forceinline__ uint4 load16(uint32_t addr) {
 // Barriers, 8 bytes each. A tile has the number n in the order of all tiles of the CTA; with n % 6 the barrier belongs to one score buffer
 // and one group of warps, so that whoever waits meets every phase of it.
 enum : uint32_t {
-    B_FULL = 0,                        // ring, at the first CTA: both CTAs' copies
-    B_EMPTY = B_FULL + kMostSlots,     // both CTAs: the products have read a slot
-    B_LOCAL = B_EMPTY + kMostSlots,    // this CTA's copies of a value tile that is cleared in part
-    B_CLEAR = B_LOCAL + kMostSlots,    // at the first CTA: cleared, by both
+    B_K_FULL = 0,                         // rings of keys and values, at the first CTA: both CTAs' copies
+    B_K_EMPTY = B_K_FULL + kMostSlots,    // both CTAs: the products have read a slot
+    B_V_FULL = B_K_EMPTY + kMostSlots,
+    B_V_EMPTY = B_V_FULL + kMostSlots,
+    B_LOCAL = B_V_EMPTY + kMostSlots,     // this CTA's copies of a value tile that is cleared in part
+    B_CLEAR = B_LOCAL + kMostSlots,       // at the first CTA: cleared, by both
     B_S = B_CLEAR + kMostSlots,        // [6] both CTAs: scores
     B_P = B_S + 6,                     // [6] at the first CTA: weights, by four warps of each
     B_REF = B_P + 6,                   // [4 quarters][2]: the reference is settled for tile n, by its warp
     B_SUM = B_REF + 8,                 // [4 quarters]: both groups' sums
     B_OUT = B_SUM + 4,                 // [4 quarters]: both groups have read the output
     B_PV = B_OUT + 4,                  // [2] both CTAs: output of tile n
-    B_Q = B_PV + 2,                    // at the first CTA: queries, by eight warps of each
-    B_END = B_Q + 1,                   // both CTAs: the unit's products
+    B_Q = B_PV + 2,                    // [2] at the first CTA: both CTAs' queries
+    B_Q_FREE = B_Q + 2,                // [2]: eight warps have left the buffer
+    B_END = B_Q_FREE + 2,                   // both CTAs: the unit's products
     B_DRAINED = B_END + 1,
     B_COUNT = B_DRAINED + 1
 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    k_attention_tile(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a,
-                     uint32_t slots, int32_t *error_word) {
+    k_attention_tile(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ AttnArgs a, uint32_t tile_rows, uint32_t slots, int32_t *error_word) {
     using namespace umma;
     using G = Tile<D>;
     extern __shared__ uint8_t raw[];
@@ -152,29 +155,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
     __shared__ Cut cuts[2];
-    __shared__ Walk walks[8][2];
+    __shared__ Walk walks[8];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster_rank(), piece = blockIdx.x >> 1;
-    const uint32_t base = (smem_addr(raw) + 1023) & ~1023u, q_s = base, ring = q_s + G::QB * G::Q_BYTES;
-    unsigned long long *at = reinterpret_cast<unsigned long long *>(raw + (ring + slots * G::SLOT - smem_addr(raw)));
+    const uint32_t base = (smem_addr(raw) + 1023) & ~1023u, q_s = base, ring_k = q_s + G::QB * G::Q_BYTES, ring_v = ring_k + slots * G::SLOT;
+    unsigned long long *at = reinterpret_cast<unsigned long long *>(raw + (ring_v + slots * G::SLOT - smem_addr(raw)));
     const uint32_t b0 = smem_addr(bars);
     auto bar = [&](uint32_t i) { return b0 + i * 8; };
     if (tid == 0) {
         dead = 0;
-        for (uint32_t i = 0; i < kMostSlots; ++i) {
-            bar_init(bar(B_FULL + i), 1);
-            bar_init(bar(B_EMPTY + i), 1);
-            bar_init(bar(B_LOCAL + i), 1);
-            bar_init(bar(B_CLEAR + i), 2);
-        }
+        for (uint32_t i = B_K_FULL; i < B_CLEAR; ++i) bar_init(bar(i), 1);
+        for (uint32_t i = 0; i < kMostSlots; ++i) bar_init(bar(B_CLEAR + i), 2);
         for (uint32_t i = 0; i < 6; ++i) {
             bar_init(bar(B_S + i), 1);
             bar_init(bar(B_P + i), 8);
         }
         for (uint32_t i = 0; i < 8; ++i) bar_init(bar(B_REF + i), 1);
         for (uint32_t i = 0; i < 8; ++i) bar_init(bar(B_SUM + i), 2);  // and B_OUT
-        bar_init(bar(B_PV), 1);
-        bar_init(bar(B_PV + 1), 1);
-        bar_init(bar(B_Q), 16);
+        for (uint32_t i = 0; i < 2; ++i) {
+            bar_init(bar(B_PV + i), 1);
+            bar_init(bar(B_Q + i), 1);
+            bar_init(bar(B_Q_FREE + i), 8);
+        }
         bar_init(bar(B_END), 1);
         bar_init(bar(B_DRAINED), 1);
         bar_init_fence();
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t tmem = tmem_slot;
     pdl_launch();
     pdl_wait();
-    lay_line(a, at, scan, reinterpret_cast<uint32_t *>(raw), error_word);
+    lay_line(a, at, scan, reinterpret_cast<Listed *>(raw), error_word);
     const Line line{a, at, a.op.n_requests};
     const Cuts cut = cuts_of(at[a.op.n_requests], gridDim.x >> 1, a.least);
     Walk w;
@@ -207,65 +208,65 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         return key0 < w.u.lo || key0 + kTileKeys > w.u.hi;
     };
     bool ok = true;
-    if (warp >= kLoadWarp) {
+    if (warp >= kKeyWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
-        if (warp == kLoadWarp) {
-            // A lane per box of a key tile; the CTAs take the boxes of 64 keys each, and half the dimensions of all values.
-            const uint32_t boxes = kTileKeys / a.box, k_bytes = a.box * D * 2, v_bytes = a.box * D;
-            uint32_t n = 0, slot = 0, round = 0;  // slots filled, and where that leaves the ring
+        if (warp == kKeyWarp || warp == kValueWarp) {
+            // A warp copies the keys, another the values, a lane per box of a tile; the CTAs take the boxes of 64 keys each, and half
+            // the dimensions of all values.
+            const bool keys = warp == kKeyWarp;
+            const uint32_t boxes = kTileKeys / a.box, box_bytes = a.box * D * (keys ? 2 : 1), both = a.box * D * 2;  // both CTAs' bytes of a box
+            const uint32_t full0 = bar(keys ? B_K_FULL : B_V_FULL), empty0 = bar(keys ? B_K_EMPTY : B_V_EMPTY), ring = keys ? ring_k : ring_v;
+            const uint32_t box = lane % 8;  // of a tile, the one that this lane copies
+            const bool own = lane < 8 && (!keys || box / (boxes / 2) == rank);
+            const uint32_t dst0 = ring + (keys ? box % (boxes / 2) : box) * box_bytes;
+            uint32_t slot = 0, round = 0;
             for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
                 const int32_t *table = table_row(a, w.at.request);
-                const uint32_t tiles = w.tile1 - w.tile0, first = (w.u.tile0 + w.tile0) * kTileKeys + lane * a.box;
-                // Order of the ring: the keys of as many tiles as there are score buffers, then values and keys in turn. A warp holds the table's entries
-                // of four tiles, eight lanes for a tile's boxes (INT32_MIN: no row sees what the box holds), and the next four are on their way:
-                // read tile by tile they would hold up every copy.
-                auto entries = [&](uint32_t group) {
-                    const uint32_t j = group * 4 + lane / 8, token = (w.u.tile0 + w.tile0 + j) * kTileKeys + lane % 8 * a.box;
-                    return j < tiles && lane % 8 < boxes && token < w.u.hi && token + a.box > w.u.lo ? table[page_index(a, token)] : INT32_MIN;
+                const uint32_t tiles = w.tile1 - w.tile0;
+                // Where the boxes of four tiles lie, eight lanes for a tile (step INT32_MIN: no row sees what the box holds, or there is no such
+                // page). The next four are on their way: read tile by tile, the table would hold up every copy.
+                int32_t step = INT32_MIN, group = 0, entry = INT32_MIN;
+                uint32_t token = 0;
+                auto read = [&](uint32_t four) {
+                    const uint32_t j = four * 4 + lane / 8;
+                    token = (w.u.tile0 + w.tile0 + j) * kTileKeys + box * a.box;
+                    entry = j < tiles && box < boxes && token < w.u.hi && token + a.box > w.u.lo ? table[page_index(a, token)] : INT32_MIN;
                 };
-                int32_t four = entries(0), next_four = entries(1);
-                uint32_t group4 = 0;
-                auto load = [&](bool keys, uint32_t j) {
-                    const int32_t page = __shfl_sync(0xffffffffu, j / 4 == group4 ? four : next_four, j % 4 * 8 + lane % 8);
-                    const bool mine = lane < 8 && page != INT32_MIN && is_page(a, page, error_word);
-                    const uint32_t copies = __popc(__ballot_sync(0xffffffffu, mine)), token = first + j * kTileKeys;
-                    const int group = (int)((token - page_index(a, token) * a.op.kv.page_tokens) / 8);
+                read(0);
+                for (uint32_t j = 0; j < tiles; ++j) {
+                    if (j % 4 == 0) {
+                        step = entry != INT32_MIN && is_page(a, entry, error_word) ? box_step(a, entry, w.at.head) : INT32_MIN;
+                        group = (int)((token - page_index(a, token) * a.op.kv.page_tokens) / 8);
+                        read(j / 4 + 1);
+                    }
+                    const int32_t to = __shfl_sync(0xffffffffu, step, j % 4 * 8 + box), at_group = __shfl_sync(0xffffffffu, group, j % 4 * 8 + box);
+                    const uint32_t copies = __popc(__ballot_sync(0xffffffffu, lane < 8 && to != INT32_MIN));
                     const bool edge = !keys && is_edge(j);
-                    if (round > 0 && !(ok = __all_sync(0xffffffffu, bar_wait(bar(B_EMPTY + slot), (round - 1) & 1, &dead)))) return;
-                    const uint32_t full = bar(B_FULL + slot), dst = ring + slot * G::SLOT;
+                    const uint32_t full = full0 + slot * 8;
+                    if (round > 0 && !(ok = __all_sync(0xffffffffu, bar_wait(empty0 + slot * 8, (round - 1) & 1, &dead)))) break;
                     if (lane == 0) {
-                        if (edge) bar_expect(bar(B_LOCAL + slot), copies * v_bytes);
-                        if (rank == 0) {  // both CTAs' bytes: for keys and for values a box has as many
+                        if (edge) bar_expect(bar(B_LOCAL + slot), copies * box_bytes);
+                        if (rank == 0) {
                             if (edge)
                                 bar_arrive(full);
                             else
-                                bar_expect(full, copies * k_bytes);
+                                bar_expect(full, copies * both);
                         }
                     }
                     __syncwarp();
-                    const int step = box_step(a, page, w.at.head);
-                    if (mine && keys && lane / (boxes / 2) == rank)
-                        load_box_pair(dst + lane % (boxes / 2) * k_bytes, &map_k, leader_addr(full), 0, group, step);
-                    if (mine && !keys) {
-                        if (edge)
-                            load_box(dst + lane * v_bytes, &map_v, bar(B_LOCAL + slot), (int)(rank * G::VC), group, step);
+                    if (own && to != INT32_MIN) {
+                        const uint32_t dst = dst0 + slot * G::SLOT;
+                        if (keys)
+                            load_box_pair(dst, &map_k, leader_addr(full), 0, at_group, to);
+                        else if (edge)
+                            load_box(dst, &map_v, bar(B_LOCAL + slot), (int)(rank * G::VC), at_group, to);
                         else
-                            load_box_pair(dst + lane * v_bytes, &map_v, leader_addr(full), (int)(rank * G::VC), group, step);
+                            load_box_pair(dst, &map_v, leader_addr(full), (int)(rank * G::VC), at_group, to);
                     }
-                    ++n;
                     if (++slot == slots) {
                         slot = 0;
                         ++round;
                     }
-                };
-                for (uint32_t k = 0; ok && k < G::NB && k < tiles; ++k) load(true, k);
-                for (uint32_t v = 0; ok && v < tiles; ++v) {
-                    if (v / 4 != group4) {  // keys are at most three tiles ahead: in this group or the next
-                        four = next_four;
-                        next_four = entries(++group4 + 1);
-                    }
-                    load(false, v);
-                    if (ok && v + G::NB < tiles) load(true, v + G::NB);
                 }
             }
             if (!ok) {  // leave no copy in flight behind; the barriers may lack the other CTA's part, so by time
@@ -277,30 +278,39 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             // the whole warp runs the loop and one lane issues: its values are uniform
             constexpr uint32_t idesc_s = Weights<T>::idesc(kTileKeys, false), idesc_o = Weights<T>::idesc(D, true);
             const bool issuer = elect_one();
-            uint32_t next = 0, next_phase = 0, cleared = 0;  // of the ring; phases of B_CLEAR
+            uint32_t next_k = 0, k_phase = 0, next_v = 0, v_phase = 0, cleared = 0;  // of the rings; phases of B_CLEAR
             uint32_t units = 0, q_now = q_s, s6 = 0, p6 = 0, p6_phase = 0, buffer_s = 0, buffer_p = 0, pv = 0;
-            auto take = [&](bool edge) {  // the next slot, once it is full
-                const uint32_t slot = next;
-                ok = ok && __all_sync(0xffffffffu, bar_wait(bar(B_FULL + slot), next_phase, &dead));
+            auto take_keys = [&]() {  // the next slot, once it is full
+                const uint32_t slot = next_k;
+                ok = ok && __all_sync(0xffffffffu, bar_wait(bar(B_K_FULL + slot), k_phase, &dead));
+                if (++next_k == slots) {
+                    next_k = 0;
+                    k_phase ^= 1;
+                }
+                return slot;
+            };
+            auto take_values = [&](bool edge) {
+                const uint32_t slot = next_v;
+                ok = ok && __all_sync(0xffffffffu, bar_wait(bar(B_V_FULL + slot), v_phase, &dead));
                 if (edge) {
                     ok = ok && __all_sync(0xffffffffu, bar_wait<BAR_PAIR>(bar(B_CLEAR + slot), cleared >> slot & 1, &dead));
                     cleared ^= 1u << slot;
                 }
-                if (++next == slots) {
-                    next = 0;
-                    next_phase ^= 1;
+                if (++next_v == slots) {
+                    next_v = 0;
+                    v_phase ^= 1;
                 }
                 return slot;
             };
             auto scores = [&](uint32_t slot) {  // S = Q K^T of the next tile
                 if (issuer) {
-                    const uint64_t dq = desc_rows(q_now, 1024), dk = desc_rows(ring + slot * G::SLOT, D * 16);
+                    const uint64_t dq = desc_rows(q_now, 1024), dk = desc_rows(ring_k + slot * G::SLOT, D * 16);
                     const uint32_t d = tmem + G::S + buffer_s * kTileKeys;
 #pragma unroll
                     for (uint32_t k = 0; k < D / 16; ++k)
                         mma_f16_pair(d, dq + (k / 4 * (kTileRows * 128) + k % 4 * 32) / 16, dk + (k / 4 * 1024 + k % 4 * 32) / 16, idesc_s, k > 0);
                     commit_pair(bar(B_S + s6));
-                    commit_pair(bar(B_EMPTY + slot));
+                    commit_pair(bar(B_K_EMPTY + slot));
                 }
                 __syncwarp();
                 s6 = s6 == 5 ? 0 : s6 + 1;
@@ -309,26 +319,28 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
                 const uint32_t tiles = w.tile1 - w.tile0;
                 if (!tiles) continue;
-                q_now = q_s + units % G::QB * G::Q_BYTES;
-                if (!(ok = __all_sync(0xffffffffu, bar_wait<BAR_PAIR>(bar(B_Q), units++ & 1, &dead)))) break;
+                const uint32_t q_buffer = units % G::QB;
+                q_now = q_s + q_buffer * G::Q_BYTES;
+                if (!(ok = __all_sync(0xffffffffu, bar_wait(bar(B_Q + q_buffer), units / G::QB & 1, &dead)))) break;
+                ++units;
                 for (uint32_t j = 0; ok && j < G::NB && j < tiles; ++j) {
-                    const uint32_t slot = take(false);
+                    const uint32_t slot = take_keys();
                     fence_after();
                     if (ok) scores(slot);
                 }
                 for (uint32_t j = 0; ok && j < tiles; ++j) {  // O += P V
                     // both operands are there long before the weights
-                    const uint32_t slot = take(is_edge(j)), keys = j + G::NB < tiles ? take(false) : 0;
+                    const uint32_t slot = take_values(is_edge(j)), keys = j + G::NB < tiles ? take_keys() : 0;
                     ok = ok && __all_sync(0xffffffffu, bar_wait<BAR_PAIR_TURN>(bar(B_P + p6), p6_phase, &dead));
                     if (!ok) break;
                     fence_after();
                     if (issuer) {
-                        const uint64_t dv = desc_columns(ring + slot * G::SLOT, G::VW * 2, G::V_GROUP, G::VW * 16);
+                        const uint64_t dv = desc_columns(ring_v + slot * G::SLOT, G::VW * 2, G::V_GROUP, G::VW * 16);
                         const uint32_t p = tmem + G::S + buffer_p * kTileKeys;
 #pragma unroll
                         for (uint32_t k = 0; k < kTileKeys / 16; ++k)
                             mma_f16_ts_pair(tmem + G::O, p + k * 8, dv + k * (2 * G::V_GROUP / 16), idesc_o, j > 0 || k > 0);
-                        commit_pair(bar(B_EMPTY + slot));
+                        commit_pair(bar(B_V_EMPTY + slot));
                         commit_pair(bar(B_PV + (pv & 1)));
                         if (j + 1 == tiles) commit_pair(bar(B_END));
                     }
@@ -347,14 +359,29 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 bar_drain(bar(B_DRAINED), 0);
             }
             __syncwarp();
-        } else if (warp == kClearWarp) {
-            // 0 times what lies in places that no row sees is not 0 if that is no number
-            uint32_t ring0 = 0, local = 0;  // slots before the unit; phases of B_LOCAL
+        } else if (warp == kUnitWarp) {
+            // Queries of each unit: tile_rows rows (whole tokens of the head's group) by copies of 64 dimensions. And clearing of value tiles: 0 times
+            // what lies in places that no row sees is not 0 if that is no number.
+            uint32_t values0 = 0, local = 0, units = 0;  // value tiles before the unit; phases of B_LOCAL
             for (; ok && walk_unit(a.shape, line, w); walk_on(a.shape, line, w)) {
                 const uint32_t tiles = w.tile1 - w.tile0;
+                if (tiles) {
+                    const uint32_t b = units % G::QB, full = bar(B_Q + b);
+                    if (units >= G::QB && !(ok = __all_sync(0xffffffffu, bar_wait(bar(B_Q_FREE + b), (units / G::QB - 1) & 1, &dead)))) break;
+                    if (lane == 0 && rank == 0) bar_expect(full, 2 * tile_rows * D * 2);
+                    __syncwarp();
+                    if (lane < D / 64)
+                        asm volatile(
+                            "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %3, %4, %5, %6}], "
+                            "[%2];" ::"r"(q_s + b * G::Q_BYTES + lane * (kTileRows * 128)),
+                            "l"(&map_q), "r"(leader_addr(full)), "r"(0),
+                            "r"((int)(w.q.q0 + divide(w.u.row0 + rank * tile_rows, a.shape.by_group))), "r"(lane), "r"(w.at.head)
+                            : "memory");
+                    ++units;
+                }
                 for (uint32_t j = 0; j < tiles; ++j) {
                     if (!is_edge(j)) continue;
-                    const uint32_t slot = (ring0 + min(min(G::NB, tiles) + j, tiles) + j) % slots, key0 = (w.u.tile0 + w.tile0 + j) * kTileKeys;
+                    const uint32_t slot = (values0 + j) % slots, key0 = (w.u.tile0 + w.tile0 + j) * kTileKeys;
                     const uint32_t x = w.u.lo > key0 ? w.u.lo - key0 : 0, y = min(w.u.hi - key0, kTileKeys);  // rows [x, y) stay
                     if (!(ok = __all_sync(0xffffffffu, bar_wait(bar(B_LOCAL + slot), local >> slot & 1, &dead)))) break;
                     local ^= 1u << slot;
@@ -362,20 +389,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     for (uint32_t r = lane / pieces; r < kTileKeys; r += 32 / pieces) {
                         const uint32_t i = lane % pieces, chunk = i / (G::VW / 8), in = i % (G::VW / 8);
                         if (r < x || r >= y)
-                            store16(ring + slot * G::SLOT + (r >> 3) * G::V_GROUP + chunk * (G::VW * 16) + (r & 7) * (G::VW * 2) + in * 16,
+                            store16(ring_v + slot * G::SLOT + (r >> 3) * G::V_GROUP + chunk * (G::VW * 16) + (r & 7) * (G::VW * 2) + in * 16,
                                     make_uint4(0, 0, 0, 0));
                     }
                     proxy_fence();
                     __syncwarp();
                     if (lane == 0) bar_release_leader(leader_addr(bar(B_CLEAR + slot)));
                 }
-                ring0 += 2 * tiles;
+                values0 += tiles;
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
         const uint32_t g = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, lanes = (quarter * 32) << 16;
-        const uint32_t in = rank * kTileRows + row;  // of the unit's rows
+        const uint32_t in = rank * tile_rows + row;  // of the unit's rows
         constexpr uint32_t P = D / 16, ROWS = 32 / P;  // 16-byte pieces of half a row; rows that a warp moves at a time
         const float c = a.c;
         const f32x2 cc = pack2(c, c), one = pack2(1.f, 1.f);
@@ -390,16 +417,29 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
         };
         auto settled = [&](uint32_t tile) { return bar_wait(bar(B_REF + quarter * 2 + (tile & 1)), tile >> 1 & 1, &dead); };
-        // Where the walk stands is kept in shared memory, for each warp this unit and the next: in registers it would push scores out of them.
-        // The first turn has no unit yet, only a next one.
-        uint32_t turn = 0;
-        auto at_end = [&](const Walk &u) { return u.q.rows_new == 0xffffffffu; };
-        // the address of this lane's row of q (or out), this group's half of its dimensions
-        auto row_of = [&](const Walk &u, const void *m, uint64_t token_stride, uint64_t head_stride) {
-            const uint32_t r = u.u.row0 + in, t = r / a.shape.group;
-            return (unsigned long long)((const T *)m + (uint64_t)(u.q.q0 + t) * token_stride +
-                                        (uint64_t)(u.at.head * a.shape.group + (r - t * a.shape.group)) * head_stride + g * (D / 2));
+        // Where the walk stands is kept in shared memory: in registers it would push scores out of them.
+        Walk &u = walks[warp];
+        bool at_end = false;
+        auto walk_to = [&](bool on) {
+            __syncwarp();
+            if (lane == 0) {
+                if (on)
+                    walk_on(a.shape, line, u);
+                else
+                    u = w;
+                at_end = !walk_unit(a.shape, line, u);
+            }
+            at_end = __shfl_sync(0xffffffffu, at_end, 0);
+            __syncwarp();
         };
+        walk_to(false);
+        // the address of this lane's row of the output, this group's half of its dimensions
+        auto out_row = [&]() {
+            const uint32_t r = u.u.row0 + in, t = divide(r, a.shape.by_group);
+            return (unsigned long long)((T *)a.op.out + (uint64_t)(u.q.q0 + t) * a.op.out_token_stride +
+                                        (uint64_t)(u.at.head * a.shape.group + (r - t * a.shape.group)) * a.op.out_head_stride + g * (D / 2));
+        };
+        auto head_in = [&](uint32_t r) { return r - divide(r, a.shape.by_group) * a.shape.group; };
         // This warp's half (g) of its 32 rows of a buffer of queries: piece i of 16 bytes of this lane, neighbours in a row by neighbouring lanes.
         auto piece_of = [&](uint32_t buffer, uint32_t i, uint32_t &at_row) {
             at_row = i * ROWS + lane / P;
@@ -411,58 +451,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             asm volatile("" : "+r"(b));  // addresses formed where they are used, not kept through the tiles
             return b;
         };
-        constexpr uint32_t at_once = P < 8 ? P : 8;
-        auto fetch = [&](const Walk &u, uint32_t i0, uint4(&x)[at_once]) {
-            const unsigned long long q = row_of(u, a.op.q, a.op.q_token_stride, a.op.q_head_stride);
-            const uint32_t live_rows = __ballot_sync(0xffffffffu, in < u.u.rows);
-#pragma unroll
-            for (uint32_t i = 0; i < at_once; ++i) {
-                const uint32_t from = (i0 + i) * ROWS + lane / P;
-                const T *src = (const T *)__shfl_sync(0xffffffffu, q, from);
-                x[i] = live_rows >> from & 1 ? reinterpret_cast<const uint4 *>(src)[lane % P] : make_uint4(0, 0, 0, 0);
-            }
-        };
-        auto put = [&](uint32_t buffer, uint32_t i0, const uint4(&x)[at_once]) {
-#pragma unroll
-            for (uint32_t i = 0; i < at_once; ++i) {
-                uint32_t at_row;
-                const uint32_t d = piece_of(buffer, i0 + i, at_row);
-                store16(d, x[i]);
-            }
-        };
-        auto queries_ready = [&]() {
-            proxy_fence();
-            __syncwarp();
-            if (lane == 0) bar_release_leader(leader_addr(bar(B_Q)));
-        };
-        auto load_queries = [&](const Walk &u, uint32_t unit) {
-            const uint32_t buffer = buffer_of(unit);
-#pragma unroll 1
-            for (uint32_t i0 = 0; i0 < P; i0 += at_once) {
-                uint4 x[at_once];
-                fetch(u, i0, x);
-                put(buffer, i0, x);
-            }
-            queries_ready();
-        };
-        for (;; ++turn) {
-            const Walk &u = walks[warp][turn & 1 ^ 1];
-            Walk &then = walks[warp][turn & 1];
-            if (turn && at_end(u)) break;
-            if (lane == 0) {
-                then = turn ? u : w;
-                if (turn) walk_on(a.shape, line, then);
-                if (!walk_unit(a.shape, line, then)) then.q.rows_new = 0xffffffffu;
-            }
-            __syncwarp();
-            const uint32_t tiles = turn ? u.tile1 - u.tile0 : 0;
-            const bool whole_unit = turn && u.begins && u.ends;
-            if (turn && u.begins && !u.ends) {
+        for (; !at_end; walk_to(true)) {
+            const uint32_t tiles = u.tile1 - u.tile0;
+            const bool whole_unit = u.begins && u.ends;
+            if (u.begins && !u.ends) {
                 shares = true;
                 if (tid == 0 && rank == 0)
                     a.shared[piece] = Shared{sharers(cut, piece, u.at.start + u.u.cost), u.at.request, u.at.head, u.u.row0, u.u.rows};
             }
-            const bool live = turn && in < u.u.rows;
+            const bool live = row < tile_rows && in < u.u.rows;
             const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
             float ref = -INFINITY;
             f32x2 sums = 0;
@@ -607,12 +604,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 if (!ok) break;
             }
-            // The next unit's queries come while the last products run, if they have a buffer of their own: then its scores are formed while this
-            // unit's output is written.
-            auto next_queries = [&](uint32_t unit) {
-                if (!at_end(then) && then.tile1 > then.tile0) load_queries(then, unit);
-            };
-            if constexpr (G::QB == 2) next_queries(units + (tiles ? 1 : 0));
             if (tiles) {
                 // the unit's products, the last reference, and the other group's sums
                 ok = bar_wait(bar(B_END), units & 1, &dead) && settled(n - 1);
@@ -637,13 +628,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
             const uint32_t o = tmem + G::O + g * (D / 2) + lanes;  // this group's half of the dimensions
             if (whole_unit && !tiles) {  // no key is seen
-                const unsigned long long out = row_of(u, a.op.out, a.op.out_token_stride, a.op.out_head_stride);
+                const unsigned long long out = out_row();
                 if (live)
                     for (uint32_t i = 0; i < P; ++i) reinterpret_cast<uint4 *>(out)[i] = make_uint4(0, 0, 0, 0);
             } else if (whole_unit) {
                 float inv = 0.f;
                 if (sum != 0.f && live) {
-                    if (a.op.sinks) sum += ex2(fmaf(a.op.sinks[u.at.head * a.shape.group + (u.u.row0 + in) % a.shape.group], 1.4426950408889634f, -ref));
+                    if (a.op.sinks) sum += ex2(fmaf(a.op.sinks[u.at.head * a.shape.group + head_in(u.u.row0 + in)], 1.4426950408889634f, -ref));
                     inv = 1.0f / sum;
                 }
                 // through shared memory, where the queries were
@@ -664,7 +655,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                 }
                 __syncwarp();
-                const unsigned long long out = row_of(u, a.op.out, a.op.out_token_stride, a.op.out_head_stride);
+                const unsigned long long out = out_row();
 #pragma unroll 4
                 for (uint32_t i = 0; i < P; ++i) {
                     uint32_t from;
@@ -673,10 +664,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     if (live_rows >> from & 1) reinterpret_cast<uint4 *>(dst)[lane % P] = load16(d);
                 }
                 __syncwarp();
-            } else if (turn) {
+            } else {
                 constexpr uint32_t BR = 2 * kTileRows;
                 float *slot = a.partial + (piece * 2ull + (u.begins ? 1 : 0)) * slot_floats(BR, D);
-                if (g == 0) {
+                if (g == 0 && live) {
                     slot[in] = ref;
                     slot[BR + in] = sum;
                 }
@@ -688,16 +679,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         tmem_ld16(o + d, v);
                         tmem_ld_wait();
 #pragma unroll
-                        for (uint32_t i = 0; i < 16; i += 4) part[(d + i) / 4 * BR] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        for (uint32_t i = 0; i < 16; i += 4)
+                            if (live) part[(d + i) / 4 * BR] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                     }
             }
             fence_before();
+            proxy_fence();  // the next copy into this buffer of queries comes behind what was staged there
             __syncwarp();
             if (tiles) {
-                if (lane == 0) bar_arrive(bar(B_OUT + quarter));
+                if (lane == 0) {
+                    bar_arrive(bar(B_OUT + quarter));
+                    bar_arrive(bar(B_Q_FREE + units % G::QB));
+                }
                 ++units;
             }
-            if constexpr (G::QB == 1) next_queries(units);
         }
         if (!shares && tid == 0 && rank == 0) a.shared[piece].sharers = 0;
     }
@@ -717,15 +712,24 @@ ctox_status tile_launch(ctox_ctx *ctx, AttnArgs &a) {
     using G = Tile<D>;
     a.box = kTileKeys / 2;
     while (a.op.kv.page_tokens % a.box) a.box /= 2;
-    CUtensorMap mk, mv;
-    EX(cache_map(ctx, &mk, a.op, a.op.kv.k, a.box, D / 64));
-    EX(cache_map(ctx, &mv, a.op, a.op.kv.v, a.box, G::VC, G::VW));
+    CUtensorMap mq, mk, mv;
+    const ctox_paged_attention_op &op = a.op;
+    const uint32_t tokens = kTileRows / a.shape.group, tile_rows = tokens * a.shape.group;
+    a.shape.block_rows = 2 * tile_rows;
+    const cuuint64_t dims[5] = {64, a.shape.group, op.n_tokens, D / 64, op.kv_heads};
+    // (strides of single rows may be 0, which a map does not take)
+    const uint64_t head = op.q_head_stride ? op.q_head_stride : 8, token = op.q_token_stride ? op.q_token_stride : 8;
+    const cuuint64_t strides[4] = {head * 2, token * 2, 128, head * a.shape.group * 2};
+    const cuuint32_t box[5] = {64, a.shape.group, tokens, 1, 1};
+    EX(encode_map(ctx, &mq, op.kv.dtype, op.q, dims, strides, box, 128));
+    EX(cache_map(ctx, &mk, op, op.kv.k, a.box, D / 64));
+    EX(cache_map(ctx, &mv, op, op.kv.v, a.box, G::VC, G::VW));
     const size_t room = (size_t)ctx->max_smem_optin - 4096;  // static shared memory
     const uint32_t slots = G::slots(room, a.op.n_requests);
     const size_t smem = G::smem(slots, a.op.n_requests);
     auto kernel = k_attention_tile<T, D>;
     CTOX_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    CTOX_CUDA(ctx, launch_pdl_cluster(kernel, dim3((uint32_t)ctx->sm_count / 2 * 2), dim3(kTileThreads), smem, ctx->stream, 2, mk, mv, a, slots,
+    CTOX_CUDA(ctx, launch_pdl_cluster(kernel, dim3((uint32_t)ctx->sm_count / 2 * 2), dim3(kTileThreads), smem, ctx->stream, 2, mq, mk, mv, a, tile_rows, slots,
                                       ctx->dev_error));
     return CTOX_OK;
 }
@@ -737,8 +741,6 @@ ctox_status tile_launch(ctox_ctx *ctx, AttnArgs &a) {
 }  // namespace
 
 ctox_status launch_attention_tile(ctox_ctx *ctx, AttnArgs &a) {
-    a.shape.block_rows = kTileBlockRows;
-    a.shape.half_rows = kTileBlockRows;  // a pair's products take as long with fewer rows
     a.shape.key_shift = 7;
     return a.op.kv.dtype == CTOX_BF16 ? tile_launch<__nv_bfloat16>(ctx, a) : tile_launch<__half>(ctx, a);
 }

@@ -22,10 +22,21 @@ struct Request {
     uint32_t q0, rows_new, kv;  // first row of q, new tokens, tokens in the cache
 };
 
+// Division of numbers below 2^31 by one known on the host.
+struct Divisor {
+    uint32_t factor, shift;
+};
+inline Divisor divisor(uint32_t d) {
+    uint32_t bits = 0;
+    while ((1ull << bits) < d) ++bits;
+    return Divisor{(uint32_t)((1ull << (31 + bits)) / d + 1), 31 + bits};
+}
+CTOX_HD uint32_t divide(uint32_t x, const Divisor &d) { return (uint32_t)((unsigned long long)x * d.factor >> d.shift); }
+
 struct Shape {
     uint32_t kv_heads, group;        // query heads per KV head
+    Divisor by_group;
     uint32_t block_rows, key_shift;  // of a unit; log2 of a key tile
-    uint32_t half_rows;              // up to that many rows in a block a tile costs 1, else 2
     uint32_t overhead;               // of a unit, in tiles
     uint32_t least_rows, most_rows;  // requests with other numbers of rows (tokens x group) are not this kernel's
     uint32_t causal, window;
@@ -37,7 +48,7 @@ CTOX_HD void key_range(const Shape &s, const Request &q, uint32_t row0, uint32_t
     hi = q.kv;
     if (!s.causal) return;
     const int64_t base = (int64_t)q.kv - q.rows_new;  // keys before the first new one
-    const int64_t first = base + row0 / s.group, last = base + (row1 - 1) / s.group;
+    const int64_t first = base + divide(row0, s.by_group), last = base + divide(row1 - 1, s.by_group);
     if (last + 1 < (int64_t)hi) hi = last + 1 > 0 ? (uint32_t)(last + 1) : 0;
     if (s.window && first + 1 > (int64_t)s.window) lo = (uint32_t)(first + 1 - s.window);
     if (lo > hi) lo = hi;
@@ -52,8 +63,7 @@ struct Unit {
     uint32_t row0, rows;   // of the request's rows
     uint32_t lo, hi;       // keys
     uint32_t tile0, tiles; // first key tile, number of them
-    uint32_t weight;       // cost of a tile
-    uint32_t cost;
+    uint32_t cost;         // in tiles
 };
 CTOX_HD Unit unit_of(const Shape &s, const Request &q, uint32_t block) {
     Unit u;
@@ -63,8 +73,7 @@ CTOX_HD Unit unit_of(const Shape &s, const Request &q, uint32_t block) {
     key_range(s, q, u.row0, u.row0 + u.rows, u.lo, u.hi);
     u.tile0 = u.lo >> s.key_shift;
     u.tiles = u.hi > u.lo ? ((u.hi - 1) >> s.key_shift) + 1 - u.tile0 : 0;
-    u.weight = u.rows > s.half_rows ? 2 : 1;
-    u.cost = s.overhead + u.tiles * u.weight;
+    u.cost = s.overhead + u.tiles;
     return u;
 }
 
@@ -102,8 +111,7 @@ CTOX_HD uint32_t sharers(const Cuts &c, uint32_t first, uint64_t end) {
 CTOX_HD uint32_t tiles_before(const Shape &s, const Unit &u, uint64_t start, uint64_t x) {
     if (x >= start + u.cost) return u.tiles;
     if (x <= start + s.overhead) return 0;
-    const uint32_t t = ((uint32_t)(x - start - s.overhead) + u.weight - 1) / u.weight;
-    return t < u.tiles ? t : u.tiles;
+    return (uint32_t)(x - start - s.overhead);
 }
 
 // A place on the line and the unit there. Line: n requests, at(i) their places (at(n) the end), per_head(i) a KV head's share,
@@ -121,10 +129,10 @@ CTOX_HD uint32_t find_block(const Shape &s, const Request &q, uint64_t &off) {
     uint64_t begin = 0;
     for (uint32_t b0 = 0;; b0 += 32) {
         const uint32_t cost = b0 + lane < blocks ? unit_of(s, q, b0 + lane).cost : 0;
-        unsigned long long upto = cost;
+        uint32_t upto = cost;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long u = __shfl_up_sync(0xffffffffu, upto, o);
+            const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= (uint32_t)o) upto += u;
         }
         const uint32_t beyond = __ballot_sync(0xffffffffu, off < begin + upto);

@@ -67,7 +67,7 @@ REFUSED = [
         dict(dim=80), dict(heads=6), dict(heads=0), dict(kv_heads=0), dict(heads=1032, kv_heads=8), dict(n_requests=0), dict(n_requests=5000),
         dict(n_tokens=1 << 31), dict(max_new_tokens=1 << 31), dict(max_kv_tokens=1 << 31), dict(max_new_tokens=1 << 29), dict(scale=0.0),
         dict(scale=-1.0), dict(scale=float("inf")), dict(query_offsets=None), dict(kv_lens=None), dict(block_table=None), dict(table_rows=0),
-        dict(max_pages=0), dict(table_stride=9), dict(q=None), dict(out=None), dict(q=P + 2), dict(out=P + 8), dict(q_head_stride=12),
+        dict(max_pages=0), dict(table_stride=9), dict(q=None), dict(out=None), dict(q=P + 2), dict(out=P + 8), dict(q_head_stride=12), dict(q_head_stride=0), dict(q_token_stride=0),
         dict(out_token_stride=1), dict(kv=kv(n_pages=1 << 28)), dict(kv=kv(page_stride=16 * 512 + 8)))),
     ("ctox_paged_attention", DTYPE, dict(kv=kv(dtype=N.F32))),
     ("ctox_paged_attention", OPERATION, dict(window=5, causal=0)), ("ctox_paged_attention", OPERATION, dict(causal=2)),
@@ -129,6 +129,9 @@ struct HostLine {
 };
 // rows out: cta, request, head, block, first tile of the unit, tile0, tile1, begins, ends, sharers (where it begins and goes on)
 extern "C" long deal(const Shape *s, const Request *q, uint32_t n, uint32_t ctas, uint32_t least, uint32_t *out, long room) {
+    Shape shape = *s;
+    shape.by_group = divisor(s->group);
+    s = &shape;
     std::vector<uint64_t> at(n + 1, 0);
     for (uint32_t i = 0; i < n; ++i) {
         uint64_t cost = 0;
@@ -165,8 +168,8 @@ def deal(tmp_path_factory):
     lib.deal.restype = C.c_long
 
     def run(shape, requests, ctas, least):
-        shape = dict(shape, key_shift=shape["key_tile"].bit_length() - 1)
-        s = np.array([shape[k] for k in ("kv_heads", "group", "block_rows", "key_shift", "half_rows", "overhead", "least_rows", "most_rows",
+        shape = dict(shape, unused=0, key_shift=shape["key_tile"].bit_length() - 1)
+        s = np.array([shape[k] for k in ("kv_heads", "group", "unused", "unused", "block_rows", "key_shift", "overhead", "least_rows", "most_rows",
                                          "causal", "window")], dtype=np.uint32)
         q = np.array(requests, dtype=np.uint32).reshape(-1, 3)
         out = np.zeros((400000, 10), dtype=np.uint32)
@@ -190,7 +193,6 @@ def draw(rng):
     shape = dict(kv_heads=int(rng.integers(1, 9)), group=int(rng.integers(1, 9)), block_rows=int(rng.choice([8, 16, 128, 256])),
                  key_tile=int(rng.choice([64, 128])), overhead=int(rng.integers(1, 9)), least_rows=1, most_rows=1 << 30, causal=int(rng.random() < 0.8),
                  window=0)
-    shape["half_rows"] = 128 if shape["block_rows"] == 256 else shape["block_rows"]
     if shape["causal"] and rng.random() < 0.4:
         shape["window"] = int(rng.integers(1, 700))
     if rng.random() < 0.3:
@@ -236,19 +238,19 @@ def test_every_tile_is_dealt_once(deal, seed):
         assert parts[0][4] and parts[-1][5] and not any(p[4] for p in parts[1:]) and not any(p[5] for p in parts[:-1])
         if len(parts) > 1:
             assert parts[0][6] == len(parts)
-            assert shape["overhead"] + tiles * (2 if len(rows) > shape["half_rows"] else 1) >= 2 * least
+            assert shape["overhead"] + tiles >= 2 * least
         else:
             assert parts[0][6] == 0
 
 
 def test_long_contexts_are_dealt_evenly(deal):
-    shape = dict(kv_heads=4, group=6, block_rows=8, key_tile=64, half_rows=8, overhead=2, least_rows=1, most_rows=16, causal=1, window=0)
+    shape = dict(kv_heads=4, group=6, block_rows=8, key_tile=64, overhead=2, least_rows=1, most_rows=16, causal=1, window=0)
     got = deal(shape, [(0, 1, 32769)], 148, 4)
     loads = np.bincount(got[:, 0], weights=got[:, 6] - got[:, 5])
     assert len(loads) == 148 and loads.max() - loads.min() <= 4 and loads.sum() == 4 * 513
 
 
 def test_a_million_tokens_do_not_overflow(deal):
-    shape = dict(kv_heads=32, group=4, block_rows=8, key_tile=64, half_rows=8, overhead=2, least_rows=1, most_rows=16, causal=1, window=0)
+    shape = dict(kv_heads=32, group=4, block_rows=8, key_tile=64, overhead=2, least_rows=1, most_rows=16, causal=1, window=0)
     got = deal(shape, [(0, 1, 1 << 24)] * 300, 148, 4)  # 2.5e9 tiles
     assert int((got[:, 6] - got[:, 5]).sum()) == 300 * 32 * (1 << 18)
