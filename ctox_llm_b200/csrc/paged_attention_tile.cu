@@ -15,8 +15,6 @@
 #include "paged_attention.cuh"
 #include "f32x2.cuh"
 
-#include <type_traits>
-
 namespace ctox {
 namespace paged {
 namespace {
@@ -49,52 +47,15 @@ struct Weights;
 template <>
 struct Weights<__nv_bfloat16> {
     static constexpr float limit = 1152921504606846976.f;  // 2^60
-    // 2^f over [-1/2, 1/2] as 1 + f (c1 + f (c2 + ...)): largest relative error 1.0e-4, against 2^-9 of a weight's rounding
-    static constexpr int terms = 3;
-    __device__ static constexpr float c(int i) { return i == 0 ? 0.6932829022407532f : i == 1 ? 0.2422109693288803f : 0.05500893294811249f; }
     __host__ __device__ static constexpr uint32_t idesc(uint32_t n, bool b_mn) { return umma::idesc_bf16_mn(2 * kTileRows, n, false, b_mn); }
 };
 template <>
 struct Weights<__half> {
     static constexpr float limit = 32768.f;  // no weight above the type's 65504
-    // the same with 2.9e-6, against 2^-12
-    static constexpr int terms = 4;
-    __device__ static constexpr float c(int i) {
-        return i == 0 ? 0.6931241750717163f : i == 1 ? 0.24024099111557007f : i == 2 ? 0.055906426161527634f : 0.009582852944731712f;
-    }
     __host__ __device__ static constexpr uint32_t idesc(uint32_t n, bool b_mn) {
         return Weights<__nv_bfloat16>::idesc(n, b_mn) & ~((1u << 7) | (1u << 10));  // the types' fields: 0 for f16
     }
 };
-
-// 2^x of two values without the special-function unit, which has 16 lanes per cycle for 128 rows of 128 scores: the pipes
-// for multiplications take a quarter of them. x is cut into a whole number (added to 1.5 * 2^23 it is in the low bits) and the rest
-// in [-1/2, 1/2], for which a polynomial, fitted for the least largest relative error, is near enough to what the type keeps; the
-// whole number then goes into the exponent. Below 2^-127 the result is 0, exactly: there the polynomial is 1. From 2^127 on it is 2^127,
-// and what is no number stays none or becomes large: either makes the tile's sum too large, and the tile is formed again by ex2.
-__device__ __forceinline__ float clamp_exponent(float x) {
-    asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n\tmin.NaN.f32 %0, %0, 0f42FE0000;" : "+f"(x));  // -127, 127
-    return x;
-}
-template <typename T>
-__device__ __forceinline__ void exp2_pair(f32x2 v, float &a, float &b) {
-    using W = Weights<T>;
-    unpack2(v, a, b);
-    v = pack2(clamp_exponent(a), clamp_exponent(b));
-    const f32x2 one = pack2(1.f, 1.f), magic = pack2(12582912.f, 12582912.f), minus_magic = pack2(-12582912.f, -12582912.f),
-                minus_one = pack2(-1.f, -1.f);
-    const f32x2 t = fma2(v, one, magic);  // rounds to a whole number
-    const f32x2 f = fma2(fma2(t, one, minus_magic), minus_one, v);
-    f32x2 y = pack2(W::c(W::terms - 1), W::c(W::terms - 1));
-#pragma unroll
-    for (int i = W::terms - 2; i >= 0; --i) y = fma2(y, f, pack2(W::c(i), W::c(i)));
-    y = fma2(y, f, one);
-    float ta, tb;
-    unpack2(t, ta, tb);
-    unpack2(y, a, b);
-    a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
-    b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
-}
 
 // Operands of swizzled rows of `width` bytes: `group` bytes from eight rows (keys) to the next eight; keys run along n (128 bytes), or along
 // k with `atom` bytes from a row's dimensions to the next ones.
@@ -104,11 +65,6 @@ __device__ __forceinline__ uint64_t desc_rows(uint32_t addr, uint32_t group) {
 __device__ __forceinline__ uint64_t desc_columns(uint32_t addr, uint32_t width, uint32_t group, uint32_t atom) {
     return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(atom >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) |
            ((width == 128 ? 2ull : 4ull) << 61);
-}
-// The compiler forms these before the next load from tensor memory: left to itself it puts them off until four loads are live, and spills.
-__device__ __forceinline__ void keep16(uint32_t *p, f32x2 (&sums)[2]) {
-    asm volatile("" : "+r"(p[0]), "+r"(p[1]), "+r"(p[2]), "+r"(p[3]), "+r"(p[4]), "+r"(p[5]), "+r"(p[6]), "+r"(p[7]), "+r"(p[8]), "+r"(p[9]), "+r"(p[10]),
-                 "+r"(p[11]), "+r"(p[12]), "+r"(p[13]), "+r"(p[14]), "+r"(p[15]), "+l"(sums[0]), "+l"(sums[1]));
 }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void store16(uint32_t addr, uint4 x) {
@@ -492,10 +448,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         uint32_t p[kTileKeys / 2];
                         f32x2 tile_sum;
                         // Weights against the reference, packed into p, and their sum. A quarter at a time, the next one on its way.
-                        auto weigh = [&](auto fast) {
+                        auto weigh = [&]() {
                             const float m = ref == -INFINITY ? 0.f : ref;
                             const f32x2 mm = pack2(-m, -m);
-                            f32x2 part[2] = {0, 0};
+                            f32x2 part[4] = {0, 0, 0, 0};
                             float s[2][32];
                             tmem_ld32(src, s[0]);
 #pragma unroll
@@ -503,26 +459,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                 float(&now)[32] = s[k0 / 32 & 1];
                                 tmem_ld_wait();
                                 if (k0 + 32 < kTileKeys) tmem_ld32(src + k0 + 32, s[k0 / 32 + 1 & 1]);
-                                if constexpr (!decltype(fast)::value) {
-                                    if (!whole) hide(now, k0);
-                                }
+                                if (!whole) hide(now, k0);
+#pragma unroll
+                                for (uint32_t k = 0; k < 32; k += 2) unpack2(fma2(pack2(now[k], now[k + 1]), cc, mm), now[k], now[k + 1]);
+#pragma unroll
+                                for (uint32_t k = 0; k < 32; ++k) now[k] = ex2(now[k]);
 #pragma unroll
                                 for (uint32_t k = 0; k < 32; k += 2) {
-                                    const f32x2 v = fma2(pack2(now[k], now[k + 1]), cc, mm);
-                                    float x, y;
-                                    if (decltype(fast)::value && k % 8 == 6) {
-                                        exp2_pair<T>(v, x, y);
-                                    } else {
-                                        unpack2(v, x, y);
-                                        x = ex2(x);
-                                        y = ex2(y);
-                                    }
-                                    part[k / 2 & 1] = fma2(pack2(x, y), one, part[k / 2 & 1]);
-                                    p[(k0 + k) / 2] = pack_pair<T>(x, y);
+                                    part[k / 2 & 3] = fma2(pack2(now[k], now[k + 1]), one, part[k / 2 & 3]);
+                                    p[(k0 + k) / 2] = pack_pair<T>(now[k], now[k + 1]);
                                 }
-                                keep16(p + k0 / 2, part);
                             }
-                            tile_sum = fma2(part[0], one, part[1]);
+                            tile_sum = fma2(fma2(part[0], one, part[1]), one, fma2(part[2], one, part[3]));
                             float x, y;
                             unpack2(tile_sum, x, y);
                             return x + y;
@@ -531,7 +479,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         if (whole && j > 0) {
                             // the usual tile: every key is seen, the reference stands. Whether the tile before has raised it is known by
                             // then, or waited for below.
-                            const float total = weigh(std::true_type());
+                            const float total = weigh();
                             const bool known = heard || bar_try(bar(B_REF + quarter * 2 + (n - 1 & 1)), n - 1 >> 1 & 1);
                             good = __all_sync(0xffffffffu, known && (!live || (refs[row] == ref && ref != -INFINITY && total <= Weights<T>::limit)));
                         }
@@ -542,7 +490,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                 const float now = refs[row], f = now == ref ? 1.f : ex2(ref - now);
                                 sums = mul2(sums, pack2(f, f));
                                 ref = now;
-                                const float total = weigh(std::false_type());
+                                const float total = weigh();
                                 raise = live && (!(total <= Weights<T>::limit) || ref == -INFINITY);
                             }
                             if (__any_sync(0xffffffffu, raise)) {
@@ -580,7 +528,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                     __syncwarp();
                                     if (lane == 0) bar_arrive(bar(B_REF + quarter * 2 + (n & 1)));
                                 }
-                                weigh(std::false_type());
+                                weigh();
                             }
                         }
                         if (!ok) break;
