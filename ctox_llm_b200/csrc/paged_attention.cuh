@@ -44,7 +44,7 @@ __device__ __forceinline__ const int32_t *table_row(const AttnArgs &a, uint32_t 
 }
 
 // Line places of all requests: at[0 .. n], by the whole block (`scan`: a word per warp). A request's blocks are summed by its thread,
-// but a long prompt's thousands by all threads: such requests are put down in `list` (room for n, free to use until the return).
+// but a long prompt's thousands by a warp: such requests are put down in `list` (room for n, free to use until the return).
 struct Listed {
     Request q;
     uint32_t index;
@@ -70,12 +70,14 @@ __device__ __forceinline__ void lay_line(const AttnArgs &a, unsigned long long *
         at[r + 1] = cost;
     }
     __syncthreads();
-    for (uint32_t i = 0, m = listed; i < m; ++i) {
+    for (uint32_t i = threadIdx.x >> 5, m = listed; i < m; i += blockDim.x >> 5) {
         const Request q = list[i].q;
-        const uint32_t blocks = blocks_of(a.shape, q);
+        const uint32_t blocks = blocks_of(a.shape, q), lane = threadIdx.x & 31;
         unsigned long long cost = 0;
-        for (uint32_t b = threadIdx.x; b < blocks; b += blockDim.x) cost += unit_of(a.shape, q, b).cost;
-        if (cost) atomicAdd(&at[list[i].index + 1], cost);
+        for (uint32_t b = lane; b < blocks; b += 32) cost += unit_of(a.shape, q, b).cost;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
+        if (lane == 0) at[list[i].index + 1] = cost;
     }
     __syncthreads();
     unsigned long long mine = 0;
