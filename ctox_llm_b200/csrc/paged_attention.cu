@@ -552,9 +552,13 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
     a.shape.by_group = divisor(a.shape.group);
     const DeviceGuard guard(ctx->device);
     CTOX_CUDA(ctx, guard.error());
-    // Only the device knows how many rows a request has; the host knows the most, and that a token has `group`.
+    // Only the device knows how many rows a request has; the host knows the most, and that a token has `group`. Where some may have
+    // many, the kernel for many takes all, unless the cache that the others may read, by the bounds that the host knows, is large: a
+    // second kernel costs about 15 us, and reads the cache a third faster. (26 requests, at most 713 MB, 156 MB in fact: 135 us with one
+    // kernel, 150 with two; 16 requests, 819 and 201 MB: 189 and 179; 250 requests, 4.4 and 1.3 GB: 430 and 304.)
     const uint64_t most = (uint64_t)op->max_new_tokens * a.shape.group;
-    const bool many = most > kFewRows, few = !many || (op->n_requests > 1 && a.shape.group <= kFewRows);
+    const uint64_t cache = 4ull * op->n_requests * op->max_kv_tokens * op->kv_heads * op->dim;
+    const bool many = most > kFewRows, few = !many || (op->n_requests > 1 && a.shape.group <= kFewRows && cache > (768ull << 20));
     MergePart parts[2] = {};
     uint32_t n_parts = 0;
     auto merged = [&](uint32_t pieces, uint32_t slot_rows) {  // where not even the longest unit that there can be is cut, there is nothing to merge
