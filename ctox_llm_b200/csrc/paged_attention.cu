@@ -358,19 +358,19 @@ constexpr uint32_t kMergeThreads = 256;
 struct MergePart {
     const Shared *shared;
     const float *partial;
-    uint32_t block_rows, pieces;
+    uint32_t slot_rows, rows, pieces;  // rows: the most that a unit has
 };
 
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) k_attention_merge(const __grid_constant__ AttnArgs a, MergePart part0, MergePart part1) {
     __shared__ float top[kMostCtas][16], sum[kMostCtas][16];
     const uint32_t D = a.op.dim, per = 4 * kMergeThreads / D;
-    // blocks of the first part, then of the second: for each piece as many as its rows want
-    const uint32_t slices0 = (part0.block_rows + per - 1) / per, blocks0 = part0.pieces * slices0;
+    // Blocks of the first part, then of the second: a block per piece for the first rows, then for the next ones. Neighbours start on one SM,
+    // which would otherwise read all parts of a unit.
+    const uint32_t blocks0 = part0.pieces * ((part0.rows + per - 1) / per);
     const bool second = blockIdx.x >= blocks0;
     const MergePart p = second ? part1 : part0;
-    const uint32_t BR = p.block_rows, slices = second ? (BR + per - 1) / per : slices0, block = second ? blockIdx.x - blocks0 : blockIdx.x;
-    const uint32_t piece = block / slices, row_first = block % slices * per;
+    const uint32_t BR = p.slot_rows, block = second ? blockIdx.x - blocks0 : blockIdx.x, piece = block % p.pieces, row_first = block / p.pieces * per;
     pdl_launch();
     pdl_wait();
     const Shared s = p.shared[piece];
@@ -564,7 +564,7 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
     auto merged = [&](uint32_t pieces, uint32_t slot_rows) {  // where not even the longest unit that there can be is cut, there is nothing to merge
         const uint64_t longest = a.shape.overhead + ((((uint64_t)op->max_kv_tokens - 1) >> a.shape.key_shift) + 1);
         if (longest <= 0xffffffffu && keeps_whole((uint32_t)longest, a.least)) return;
-        parts[n_parts++] = MergePart{a.shared, a.partial, slot_rows, pieces};
+        parts[n_parts++] = MergePart{a.shared, a.partial, slot_rows, most < slot_rows ? (uint32_t)most : slot_rows, pieces};
     };
     if (few) {
         a.shape.least_rows = 1;
@@ -589,7 +589,7 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
     if (n_parts) {
         const uint32_t per = 4 * kMergeThreads / op->dim;
         uint32_t grid = 0;
-        for (const MergePart &p : parts) grid += p.pieces * ((p.block_rows + per - 1) / per);
+        for (const MergePart &p : parts) grid += p.pieces * ((p.rows + per - 1) / per);
         CTOX_CUDA(ctx, op->kv.dtype == CTOX_BF16 ? launch_pdl(k_attention_merge<__nv_bfloat16>, dim3(grid), dim3(kMergeThreads), 0, ctx->stream, a, parts[0], parts[1])
                                                  : launch_pdl(k_attention_merge<__half>, dim3(grid), dim3(kMergeThreads), 0, ctx->stream, a, parts[0], parts[1]));
     }
