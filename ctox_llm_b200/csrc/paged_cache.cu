@@ -1,6 +1,8 @@
 // Bookkeeping and contents of a paged K/V cache that many requests share: pages and slots of new tokens, pages given back,
 // and a layer's queries, keys and values between their projection and attention.
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -169,149 +171,209 @@ __global__ void __launch_bounds__(kPageThreads) k_page_release(const __grid_cons
 
 struct RopeArgs {
     ctox_rope_append_op op;
+    Divisor by_page;
     double turns[128];  // of pair i per position: rope_base^(-2i / rot_dim) / 2 pi
 };
 
-__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
-    const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+// Four values on their way (nothing else writes the sources while the kernel runs), and unpacked.
+__device__ __forceinline__ uint4 fetch4(const float *p) { return __ldg(reinterpret_cast<const uint4 *>(p)); }
+template <typename S>
+__device__ __forceinline__ uint2 fetch4(const S *p) { return __ldg(reinterpret_cast<const uint2 *>(p)); }
+template <typename S>
+struct Four { using type = uint2; };
+template <>
+struct Four<float> { using type = uint4; };
+template <typename S>
+__device__ __forceinline__ void unpack4(uint4 w, float *v) {
+    v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&v)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void load8(const __half *p, float (&v)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+template <typename S>
+__device__ __forceinline__ void unpack4(uint2 w, float *v) {
+    if constexpr (std::is_same_v<S, __half>) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    } else {
+        v[0] = __uint_as_float(w.x << 16), v[1] = __uint_as_float(w.x & 0xffff0000u);
+        v[2] = __uint_as_float(w.y << 16), v[3] = __uint_as_float(w.y & 0xffff0000u);
     }
 }
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
 
-// Eight dimensions from d0 on behind the norm, if there is one.
-__device__ __forceinline__ void normed8(const float (&v)[8], const float *w, uint32_t d0, float inv, float offset, float (&r)[8]) {
-    float f[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
-    if (w) {
-        load8(w + d0, f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = inv * (offset + f[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = v[j] * f[j];
+template <typename T>
+__device__ __forceinline__ void store4(T *p, const float *v) {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]));
 }
 
-// One CTA per token (and share of its heads): the turn of every pair of dimensions once into shared memory, then
-// D / 8 lanes per head with eight dimensions each, the norm's sum through shuffles.
-template <typename S, typename T, int D>
-__global__ void __launch_bounds__(256) k_rope_append(const __grid_constant__ RopeArgs a, int32_t *error_word) {
+// y = x / rms(x) * (w + offset), then pairs (u, w) -> (u cos - w sin, w cos + u sin); 32-bit throughout, one rounding at the end.
+// A CTA takes a few neighbouring tokens, all CTAs of a wave alike many. Once for each it forms the turns of the pairs (64-bit arithmetic where whole
+// turns leave, and a sine that all heads share) and the addresses of queries, keys and values in shared memory; then D / 8 lanes per
+// head with eight dimensions each, the norm's sum through shuffles. Both partners of a half-split pair are one lane's, so nothing is read twice.
+// Bound by latency and instructions as much as by memory: 4099 tokens of 16 + 4 + 4 heads of 128, 16 bits, take 16.7 us (3.1 TB/s), 19.3 with
+// one token's words under way per lane instead of two, 18.1 with CTAs in waves of unequal fill; 2475 tokens of 24 + 4 + 4 heads of 256 with norms
+// 25.6 us (3.2 TB/s), 30.1 in 2.1 waves. With few tokens several CTAs share a token's heads: 16 tokens take 4.0 us, mostly launch and dependent reads.
+constexpr uint32_t kRopeThreads = 256, kRopeTurns = 512, kRopeTokens = 8, kRopeResident = 4, kRopeTrips = 2;
+struct RopeRow {  // the heads of one kind of a token
+    const void *x;
+    void *out;
+};
+
+template <typename S, typename T, int D, bool NORM>
+__global__ void __launch_bounds__(kRopeThreads, kRopeResident) k_rope_append(const __grid_constant__ RopeArgs a, int32_t *error_word) {
     constexpr uint32_t L = D / 8;  // lanes of a head
-    __shared__ float2 turn[128];   // cosine and sine of each pair
+    __shared__ __align__(16) float2 turns[kRopeTurns];  // cosine and sine of each pair of each token
+    __shared__ __align__(16) float weights[NORM ? 2 : 1][NORM ? D : 1];  // of the norms of queries and keys, offset added
+    __shared__ RopeRow rows[kRopeTokens][3];
     const ctox_rope_append_op &op = a.op;
-    const uint32_t token = blockIdx.x, pairs = op.rot_dim / 2;
+    const uint32_t token0 = (uint64_t)blockIdx.x * op.tokens / gridDim.x, tokens = (uint64_t)(blockIdx.x + 1) * op.tokens / gridDim.x - token0;
+    const uint32_t pairs = op.rot_dim / 2;
     pdl_launch();
     pdl_wait();
-    for (uint32_t p = threadIdx.x; p < pairs; p += blockDim.x) {
-        // whole turns leave in 64 bits: a far position times the fastest pair is thousands of turns
-        const double t = (double)op.positions[op.axis[p] * op.position_stride + token] * a.turns[p];
-        float sn, cs;
-        sincospif((float)(2.0 * (t - rint(t))), &sn, &cs);
-        turn[p] = make_float2(cs, sn);
-    }
-    const int32_t slot = op.k ? op.slots[token] : -1;
-    const bool stored = slot >= 0 && (uint32_t)slot < op.kv.n_pages * op.kv.page_tokens;
-    if (slot >= 0 && !stored && threadIdx.x == 0) bad_index(error_word);
-    const uint64_t place = stored ? (uint64_t)(slot / op.kv.page_tokens) * op.kv.page_stride +
-                                        (uint64_t)(slot % op.kv.page_tokens) * op.kv.token_stride
-                                  : 0;
-    __syncthreads();
-    const uint32_t q_heads = op.q ? op.heads : 0, heads = q_heads + (stored ? 2 * op.kv_heads : 0);
-    const uint32_t lane = threadIdx.x % L, d0 = lane * 8, rot = op.rot_dim, half = rot / 2;
-    const uint32_t step = gridDim.y * (blockDim.x / L);
-    // all lanes of a warp take the same number of trips: the norm's shuffles want them together
-    for (uint32_t first = blockIdx.y * (blockDim.x / L); first < heads; first += step) {
-        const uint32_t i = first + threadIdx.x / L;
-        const bool live = i < heads, is_q = i < q_heads, is_k = !is_q && i < q_heads + op.kv_heads;
-        const uint32_t h = is_q ? i : is_k ? i - q_heads : i - q_heads - op.kv_heads;
-        const S *x = nullptr;
-        T *out = nullptr;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live) {
-            x = is_q   ? (const S *)op.q + token * op.q_token_stride + h * op.q_head_stride
-                : is_k ? (const S *)op.k + token * op.k_token_stride + h * op.k_head_stride
-                       : (const S *)op.v + token * op.v_token_stride + h * op.v_head_stride;
-            out = is_q   ? (T *)op.q_out + token * op.q_out_token_stride + h * op.q_out_head_stride
-                  : is_k ? (T *)op.kv.k + place + h * op.kv.head_stride
-                         : (T *)op.kv.v + place + h * op.kv.head_stride;
-            load8(x + d0, v);
+    if (threadIdx.x < tokens) {
+        const uint32_t t = threadIdx.x;
+        const uint64_t token = token0 + t;
+        int32_t slot = op.k ? op.slots[token] : -1;
+        if (slot >= 0 && (uint32_t)slot >= op.kv.n_pages * op.kv.page_tokens) {
+            bad_index(error_word);
+            slot = -1;
         }
-        const float *w = is_q ? op.q_norm : is_k ? op.k_norm : nullptr;
-        float sum = 0.f;
+        const uint32_t page = slot >= 0 ? divide((uint32_t)slot, a.by_page) : 0;
+        const uint64_t place = page * op.kv.page_stride + (uint64_t)(slot >= 0 ? slot - page * op.kv.page_tokens : 0) * op.kv.token_stride;
+        rows[t][0] = RopeRow{(const S *)op.q + token * op.q_token_stride, (T *)op.q_out + token * op.q_out_token_stride};
+        rows[t][1] = RopeRow{(const S *)op.k + token * op.k_token_stride, slot >= 0 ? (T *)op.kv.k + place : nullptr};
+        rows[t][2] = RopeRow{(const S *)op.v + token * op.v_token_stride, slot >= 0 ? (T *)op.kv.v + place : nullptr};
+    }
+    if constexpr (NORM)
+        for (uint32_t i = threadIdx.x; i < 2 * D; i += kRopeThreads) {
+            const float *w = i < D ? op.q_norm : op.k_norm;
+            weights[i / D][i % D] = w ? op.norm_offset + w[i % D] : 1.f;
+        }
+    // Half-split pairs by fours (`paired`): a lane's four turns are two words of 16 bytes that neighbouring lanes have side by side.
+    const bool adjacent = op.pairing == CTOX_ROPE_ADJACENT, paired = !adjacent && pairs % 4 == 0;
+    for (uint32_t i = threadIdx.x; i < tokens * pairs; i += kRopeThreads) {
+        const uint32_t t = i / pairs, p = i - t * pairs;
+        // a far position times the fastest pair is thousands of turns
+        const double x = (double)op.positions[op.axis[p] * op.position_stride + token0 + t] * a.turns[p];
+        float sn, cs;
+        sincospif((float)(2.0 * (x - rint(x))), &sn, &cs);
+        turns[t * pairs + (paired ? ((p & 3) >> 1) * (pairs / 2) + (p >> 2) * 2 + (p & 1) : p)] = make_float2(cs, sn);
+    }
+    __syncthreads();
+    const uint32_t q_heads = op.q ? op.heads : 0, heads = q_heads + (op.k ? 2 * op.kv_heads : 0);
+    // A lane's dimensions are two runs of four. Where pairs are half-split by fours, the second run holds the partners of the first.
+    const uint32_t lane = threadIdx.x % L, rot = op.rot_dim, half = pairs;
+    const bool both = paired && 4 * lane < half, turned = both || (!paired && 8 * lane < rot);
+    const uint32_t d0 = both ? 4 * lane : 8 * lane, d1 = both ? d0 + half : d0 + 4;
+    constexpr uint32_t AT_ONCE = kRopeThreads / L;
+    // All lanes of a warp take the same number of trips: the norm's shuffles want them together.
+    for (uint32_t first = blockIdx.y * AT_ONCE + threadIdx.x / 32 * (32 / L); first < heads; first += gridDim.y * AT_ONCE) {
+        const uint32_t i = first + threadIdx.x % 32 / L;
+        const bool here = i < heads;
+        const uint32_t kind = i < q_heads ? 0 : i < q_heads + op.kv_heads ? 1 : 2;
+        const uint32_t h = kind == 0 ? i : kind == 1 ? i - q_heads : i - q_heads - op.kv_heads;
+        const uint64_t x_head = h * (kind == 0 ? op.q_head_stride : kind == 1 ? op.k_head_stride : op.v_head_stride);
+        const uint64_t out_head = h * (kind == 0 ? op.q_out_head_stride : op.kv.head_stride);
+        const bool normed = NORM && (kind == 0 ? op.q_norm : kind == 1 ? op.k_norm : nullptr) != nullptr;
+        float w[8];
+        if constexpr (NORM) {
+            const float *row = weights[kind == 1];
+            *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(row + d0);
+            *reinterpret_cast<float4 *>(w + 4) = *reinterpret_cast<const float4 *>(row + d1);
+        }
+        for (uint32_t t0 = 0; t0 < tokens; t0 += kRopeTrips) {
+            typename Four<S>::type in[kRopeTrips][2] = {};
+            T *out[kRopeTrips];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += v[j] * v[j];
+            for (uint32_t n = 0; n < kRopeTrips; ++n) {
+                out[n] = nullptr;
+                if (t0 + n >= tokens || !here) continue;
+                const RopeRow row = rows[t0 + n][kind];
+                if (!row.out) continue;
+                out[n] = (T *)row.out + out_head;
+                const S *x = (const S *)row.x + x_head;
+                in[n][0] = fetch4(x + d0);
+                in[n][1] = fetch4(x + d1);
+            }
 #pragma unroll
-        for (uint32_t o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (!live) continue;
-        const float inv = 1.0f / sqrtf(sum / (float)D + op.norm_eps);
-        float r[8];
-        normed8(v, w, d0, inv, op.norm_offset, r);
-        if ((is_q || is_k) && d0 < rot) {
-            if (op.pairing == CTOX_ROPE_ADJACENT) {
+            for (uint32_t n = 0; n < kRopeTrips; ++n) {
+                if (t0 + n >= tokens) break;
+                float v[8];
+                unpack4<S>(in[n][0], v);
+                unpack4<S>(in[n][1], v + 4);
+                float inv = 1.f;
+                if constexpr (NORM) {
+                    float sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    if (d0 + j >= rot) continue;
-                    const float2 t = turn[(d0 + j) / 2];
-                    const float u = r[j], y = r[j + 1];
-                    r[j] = u * t.x - y * t.y;
-                    r[j + 1] = y * t.x + u * t.y;
+                    for (int j = 0; j < 8; ++j) sum = fmaf(v[j], v[j], sum);
+#pragma unroll
+                    for (uint32_t o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (normed) {
+                        inv = rsqrtf(sum * (1.f / D) + op.norm_eps);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] *= inv * w[j];
+                    }
                 }
-            } else if (half % 8 == 0) {  // eight partners lie together
-                const bool low = d0 < half;
-                const uint32_t e0 = low ? d0 + half : d0 - half, p0 = low ? d0 : e0;
-                float y[8];
-                load8(x + e0, y);
-                normed8(y, w, e0, inv, op.norm_offset, y);
+                if (!out[n]) continue;
+                if (turned && kind < 2) {
+                    const float2 *turn = turns + (t0 + n) * pairs;
+                    if (both) {
+                        const float4 *z = reinterpret_cast<const float4 *>(turn) + lane;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float2 t = turn[p0 + j];
-                    r[j] = low ? r[j] * t.x - y[j] * t.y : r[j] * t.x + y[j] * t.y;
-                }
-            } else {
+                        for (int j = 0; j < 4; j += 2) {
+                            const float4 two = z[j / 2 * (pairs / 4)];
+                            const float a0 = v[j], a1 = v[j + 1], b0 = v[j + 4], b1 = v[j + 5];
+                            v[j] = a0 * two.x - b0 * two.y;
+                            v[j + 4] = b0 * two.x + a0 * two.y;
+                            v[j + 1] = a1 * two.z - b1 * two.w;
+                            v[j + 5] = b1 * two.z + a1 * two.w;
+                        }
+                    } else if (adjacent) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t d = d0 + j;
-                    if (d >= rot) continue;
-                    const bool low = d < half;
-                    const uint32_t other = low ? d + half : d - half;
-                    const float y = as_float(x[other]) * (w ? inv * (op.norm_offset + w[other]) : 1.0f);
-                    const float2 t = turn[low ? d : other];
-                    r[j] = low ? r[j] * t.x - y * t.y : r[j] * t.x + y * t.y;
+                        for (int j = 0; j < 8; j += 2) {
+                            if (d0 + j >= rot) continue;
+                            const float2 z = turn[(d0 + j) / 2];
+                            const float u = v[j], y = v[j + 1];
+                            v[j] = u * z.x - y * z.y;
+                            v[j + 1] = y * z.x + u * z.y;
+                        }
+                    } else {
+                        const S *x = (const S *)rows[t0 + n][kind].x + x_head;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t d = d0 + j;
+                            if (d >= rot) continue;
+                            const bool lower = d < half;
+                            const uint32_t e = lower ? d + half : d - half;
+                            float y = as_float(x[e]);
+                            if constexpr (NORM)
+                                if (normed) y *= inv * weights[kind][e];
+                            const float2 z = turn[lower ? d : e];
+                            v[j] = lower ? v[j] * z.x - y * z.y : v[j] * z.x + y * z.y;
+                        }
+                    }
                 }
+                store4<T>(out[n] + d0, v);
+                store4<T>(out[n] + d1, v + 4);
             }
         }
-        *reinterpret_cast<uint4 *>(out + d0) =
-            make_uint4(pack_pair<T>(r[0], r[1]), pack_pair<T>(r[2], r[3]), pack_pair<T>(r[4], r[5]), pack_pair<T>(r[6], r[7]));
     }
 }
 
+template <typename S, typename T, bool NORM>
+cudaError_t launch_rope(ctox_ctx *ctx, const RopeArgs &a) {
+    const uint32_t per_trip = kRopeThreads / (a.op.dim / 8), heads = (a.op.q ? a.op.heads : 0) + (a.op.k ? 2 * a.op.kv_heads : 0);
+    const uint32_t pairs = a.op.rot_dim / 2, sms = (uint32_t)ctx->sm_count;
+    // even shares, in as few whole waves of CTAs as their turns and addresses have room for
+    const uint32_t room = pairs && kRopeTurns / pairs < kRopeTokens ? kRopeTurns / pairs : kRopeTokens, wave = kRopeResident * sms;
+    const uint32_t waves = (a.op.tokens + wave * room - 1) / (wave * room);
+    const dim3 grid(std::min(a.op.tokens, waves * wave), a.op.tokens < 2 * sms ? (heads + per_trip - 1) / per_trip : 1);
+    auto kernel = a.op.dim == 64 ? k_rope_append<S, T, 64, NORM> : a.op.dim == 128 ? k_rope_append<S, T, 128, NORM> : k_rope_append<S, T, 256, NORM>;
+    return launch_pdl(kernel, grid, dim3(kRopeThreads), 0, ctx->stream, a, ctx->dev_error);
+}
 template <typename S, typename T>
 cudaError_t launch_rope(ctox_ctx *ctx, const RopeArgs &a) {
-    const uint32_t per_trip = 256 / (a.op.dim / 8);
-    const uint32_t heads = (a.op.q ? a.op.heads : 0) + (a.op.k ? 2 * a.op.kv_heads : 0);
-    const uint32_t trips = (heads + per_trip - 1) / per_trip;
-    const dim3 grid(a.op.tokens, a.op.tokens < 2 * (uint32_t)ctx->sm_count ? trips : 1);
-    auto kernel = a.op.dim == 64 ? k_rope_append<S, T, 64> : a.op.dim == 128 ? k_rope_append<S, T, 128> : k_rope_append<S, T, 256>;
-    return launch_pdl(kernel, grid, dim3(256), 0, ctx->stream, a, ctx->dev_error);
+    return a.op.q_norm || a.op.k_norm ? launch_rope<S, T, true>(ctx, a) : launch_rope<S, T, false>(ctx, a);
 }
 template <typename S>
 cudaError_t launch_rope(ctox_ctx *ctx, const RopeArgs &a) {
@@ -377,7 +439,7 @@ ctox_status ctox_rope_append(ctox_ctx *ctx, const ctox_rope_append_op *op) {
     if (op->source_dtype != CTOX_F32 && op->source_dtype != CTOX_BF16 && op->source_dtype != CTOX_F16)
         return fail(ctx, CTOX_UNSUPPORTED_DTYPE, "%s: sources of dtype %u", what, op->source_dtype);
     if (op->kv.dtype != CTOX_BF16 && op->kv.dtype != CTOX_F16) return fail(ctx, CTOX_UNSUPPORTED_DTYPE, "%s: dtype %u", what, op->kv.dtype);
-    if (op->tokens > 0x7fffffffu) return fail(ctx, CTOX_SHAPE, "%s: %u tokens", what, op->tokens);
+    if (op->tokens > 1u << 24) return fail(ctx, CTOX_SHAPE, "%s: %u tokens (up to 2^24)", what, op->tokens);
     if ((op->q && (!op->heads || op->heads > 65535)) || (op->k && (!op->kv_heads || op->kv_heads > 65535)))
         return fail(ctx, CTOX_SHAPE, "%s: %u query heads, %u KV heads", what, op->heads, op->kv_heads);
     if (op->rot_dim % 2 || op->rot_dim > op->dim) return fail(ctx, CTOX_SHAPE, "%s: %u rotated of %u dimensions", what, op->rot_dim, op->dim);
@@ -407,6 +469,7 @@ ctox_status ctox_rope_append(ctox_ctx *ctx, const ctox_rope_append_op *op) {
     if (!op->tokens) return CTOX_OK;
     RopeArgs a;
     a.op = *op;
+    a.by_page = divisor(op->k ? op->kv.page_tokens : 1);
     // rope_base^(-2i / rot_dim) as powers of one factor, in 80 bits: at most 128 roundings of 2^-64
     const long double ratio = op->rot_dim ? powl((long double)op->rope_base, -2.0L / op->rot_dim) : 1.0L;
     long double f = 1.0L / 6.283185307179586476925286766559L;

@@ -376,8 +376,8 @@ ctox_status ctox_page_release(ctox_ctx *ctx, const ctox_page_release_op *op);
  * 2i + 1. Angles are formed in 64 bits, everything else in 32, and rounded once to kv.dtype, the type of q_out.
  * Keys and values go to slots[token] (negative: not stored); what two tokens with one slot leave there is
  * undefined. q NULL: keys and values only; k and v NULL: queries only. dim 64, 128 or 256; all strides are multiples of
- * 8 elements, all matrices and norm weights aligned to 16 bytes. source_dtype: CTOX_F32, CTOX_BF16 or CTOX_F16. q_out must not overlap
- * the sources. */
+ * 8 elements, all matrices and norm weights aligned to 16 bytes. source_dtype: CTOX_F32, CTOX_BF16 or CTOX_F16. q_out and the
+ * cache must not overlap the sources. */
 enum { CTOX_ROPE_HALF = 0, CTOX_ROPE_ADJACENT = 1 };
 typedef struct {
     uint32_t tokens, heads, kv_heads, dim, rot_dim, axes, pairing, source_dtype;
