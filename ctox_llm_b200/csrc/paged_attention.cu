@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(Rows<D, NT>::NW * 32 + 32)
             if (w.begins) {
                 shares = true;
                 if (tid == 0)
-                    a.shared[blockIdx.x] = Shared{sharers(cut, blockIdx.x, w.at.start + w.u.cost), w.at.request, w.at.head, w.u.row0, w.u.rows};
+                    a.shared[blockIdx.x] = Shared{sharers(cut, blockIdx.x, w.at.start + w.u.cost), w.q.q0, w.at.head, w.u.row0, w.u.rows};
             }
         }
     }
@@ -351,9 +351,12 @@ __global__ void __launch_bounds__(Rows<D, NT>::NW * 32 + 32)
     if (!ok && lane == 0) *error_word = DEV_ERR_WAIT_TIMEOUT;
 }
 
-// What several CTAs share. Each holds the maximum, sum and output of its keys; with M the largest maximum, weights 2^(m - M) bring
-// them to one scale, in the order of the CTAs. A block takes 1024 / D rows of one unit, four dimensions per thread. The parts: units of the kernel for few rows, of the one for many.
-constexpr uint32_t kMergeThreads = 256;
+// What several CTAs share. Each holds the maximum, sum and output of its keys; with M the largest maximum so far, weights 2^(m - M) bring
+// them to one scale, four parts at a time in the order of the CTAs. A block takes 1024 / D rows of one unit, four dimensions per thread. The
+// parts: units of the kernel for few rows, of the one for many. Bound by the latency of dependent loads where few units are shared by many CTAs (one
+// session of 32768 keys: all three loads of a part leave together, 42.7 us with the attention; 46.8 with the maxima in a pass of their own),
+// by its traffic through the L2 and the start of its blocks where many are. Fewer blocks with more rows each gave 0 to 3 % there and took 8 us here.
+constexpr uint32_t kMergeThreads = 256, kMergeParts = 4;
 
 struct MergePart {
     const Shared *shared;
@@ -363,7 +366,6 @@ struct MergePart {
 
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) k_attention_merge(const __grid_constant__ AttnArgs a, MergePart part0, MergePart part1) {
-    __shared__ float top[kMostCtas][16], sum[kMostCtas][16];
     const uint32_t D = a.op.dim, per = 4 * kMergeThreads / D;
     // Blocks of the first part, then of the second: a block per piece for the first rows, then for the next ones. Neighbours start on one SM,
     // which would otherwise read all parts of a unit.
@@ -376,41 +378,45 @@ __global__ void __launch_bounds__(kMergeThreads) k_attention_merge(const __grid_
     const Shared s = p.shared[piece];
     if (!s.sharers || row_first >= s.rows) return;
     const uint64_t slot = slot_floats(BR, D);
-    auto slot_of = [&](uint32_t i) { return p.partial + ((uint64_t)(piece + i) * 2 + (i ? 0 : 1)) * slot; };
-    Request q;
-    read_request(a, s.request, q);
-    const uint32_t tid = threadIdx.x, group = a.shape.group;
-    for (uint32_t i = tid; i < s.sharers * per; i += kMergeThreads)
-        if (row_first + i % per < s.rows) {
-            const float *x = slot_of(i / per) + row_first + i % per;
-            top[i / per][i % per] = x[0];
-            sum[i / per][i % per] = x[BR];
-        }
-    __syncthreads();
-    const uint32_t in = tid % per, d4 = tid / per, row = row_first + in;
+    const uint32_t row = row_first + threadIdx.x % per, d4 = threadIdx.x / per, group = a.shape.group;
     if (row >= s.rows) return;
-    // a part that saw nothing for this row has maximum -inf and sum 0
-    float most = -INFINITY;
-    for (uint32_t i = 0; i < s.sharers; ++i) most = fmaxf(most, top[i][in]);
-    const float ref = most == -INFINITY ? 0.f : most;
+    float most = -INFINITY, all = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float all = 0.f;
-#pragma unroll 8
-    for (uint32_t i = 0; i < s.sharers; ++i) {
-        const float4 x = reinterpret_cast<const float4 *>(slot_of(i) + 2 * BR)[d4 * BR + row];
-        const float f = umma::ex2(top[i][in] - ref);
-        all = fmaf(f, sum[i][in], all);
-        if (f != 0.f) {
-            o.x = fmaf(f, x.x, o.x);
-            o.y = fmaf(f, x.y, o.y);
-            o.z = fmaf(f, x.z, o.z);
-            o.w = fmaf(f, x.w, o.w);
+    for (uint32_t i0 = 0; i0 < s.sharers; i0 += kMergeParts) {
+        float top[kMergeParts], sum[kMergeParts];
+        float4 x[kMergeParts];
+#pragma unroll
+        for (uint32_t i = 0; i < kMergeParts; ++i) {
+            top[i] = -INFINITY;
+            if (i0 + i >= s.sharers) continue;
+            const float *part = p.partial + ((uint64_t)(piece + i0 + i) * 2 + (i0 + i ? 0 : 1)) * slot;
+            top[i] = part[row];
+            sum[i] = part[BR + row];
+            x[i] = reinterpret_cast<const float4 *>(part + 2 * BR)[d4 * BR + row];
+        }
+        // a part that saw nothing for this row has maximum -inf and sum 0
+        float now = most;
+#pragma unroll
+        for (uint32_t i = 0; i < kMergeParts; ++i) now = fmaxf(now, top[i]);
+        const float ref = now == -INFINITY ? 0.f : now, before = umma::ex2(most - ref);
+        most = now;
+        all *= before;
+        o = make_float4(o.x * before, o.y * before, o.z * before, o.w * before);
+#pragma unroll
+        for (uint32_t i = 0; i < kMergeParts; ++i) {
+            const float f = umma::ex2(top[i] - ref);
+            if (f == 0.f) continue;
+            all = fmaf(f, sum[i], all);
+            o.x = fmaf(f, x[i].x, o.x);
+            o.y = fmaf(f, x[i].y, o.y);
+            o.z = fmaf(f, x[i].z, o.z);
+            o.w = fmaf(f, x[i].w, o.w);
         }
     }
-    const uint32_t r = s.row0 + row, head = s.head * group + r % group;
-    if (all != 0.f && a.op.sinks) all += umma::ex2(fmaf(a.op.sinks[head], 1.4426950408889634f, -ref));
+    const uint32_t r = s.row0 + row, token = divide(r, a.shape.by_group), head = s.head * group + r - token * group;
+    if (all != 0.f && a.op.sinks) all += umma::ex2(fmaf(a.op.sinks[head], 1.4426950408889634f, most == -INFINITY ? 0.f : -most));
     const float f = all == 0.f ? 0.f : 1.0f / all;
-    T *out = (T *)a.op.out + (uint64_t)(q.q0 + r / group) * a.op.out_token_stride + (uint64_t)head * a.op.out_head_stride + d4 * 4;
+    T *out = (T *)a.op.out + (uint64_t)(s.q0 + token) * a.op.out_token_stride + (uint64_t)head * a.op.out_head_stride + d4 * 4;
     *reinterpret_cast<uint2 *>(out) = make_uint2(pack_pair<T>(o.x * f, o.y * f), pack_pair<T>(o.z * f, o.w * f));
 }
 

@@ -10,7 +10,7 @@ namespace paged {
 // A unit that several CTAs share: the first of them writes this down, the merge reads it.
 struct Shared {
     uint32_t sharers;  // 0: none begins here
-    uint32_t request, head, row0, rows;
+    uint32_t q0, head, row0, rows;  // q0: the request's first row of q
 };
 
 struct AttnArgs {

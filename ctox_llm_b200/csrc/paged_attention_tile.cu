@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (u.begins && !u.ends) {
                 shares = true;
                 if (tid == 0 && rank == 0)
-                    a.shared[piece] = Shared{sharers(cut, piece, u.at.start + u.u.cost), u.at.request, u.at.head, u.u.row0, u.u.rows};
+                    a.shared[piece] = Shared{sharers(cut, piece, u.at.start + u.u.cost), u.q.q0, u.at.head, u.u.row0, u.u.rows};
             }
             const bool live = row < tile_rows && in < u.u.rows;
             const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
