@@ -17,7 +17,6 @@ namespace paged {
 namespace {
 
 constexpr int kStages = 3;
-constexpr uint32_t kMostCtas = 160;  // one per SM
 constexpr uint32_t kFewRows = 16;    // requests with more rows are paged_attention_tile.cu's
 
 template <int D, int NT>
@@ -544,7 +543,6 @@ ctox_status ctox_paged_attention(ctox_ctx *ctx, const ctox_paged_attention_op *o
     if (!op->workspace || !aligned16(op->workspace) || op->workspace_bytes < workspace_bytes(ctx, *op))
         return fail(ctx, CTOX_SHAPE, "%s: workspace of %llu bytes, %llu wanted, aligned to 16", what, (unsigned long long)op->workspace_bytes,
                     (unsigned long long)workspace_bytes(ctx, *op));
-    if (ctx->sm_count > (int)kMostCtas) return fail(ctx, CTOX_UNSUPPORTED_OPERATION, "%s: %d SMs", what, ctx->sm_count);
     if (!op->n_tokens || !op->max_new_tokens) return CTOX_OK;
     AttnArgs a = {};
     a.op = *op;

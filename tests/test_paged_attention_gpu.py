@@ -250,6 +250,73 @@ def test_two_streams_at_once(be):
         b.close()
 
 
+def test_two_graphs_at_once(be):
+    """Graphs of two contexts that overlap, each with a workspace of its own: units that many CTAs share."""
+    work = []
+    for i in range(2):
+        stream = torch.cuda.Stream()
+        b = ctox.B200Backend(0, stream=stream.cuda_stream)
+        c = Cache([9000 + 100 * i, 200], 2, 128, 16, "bf16", seed=i)
+        q = queries(c, 8, [4, 70], seed=i)
+        out = torch.zeros_like(q)
+        op, keep = attention_op(b, c, q, out, [4, 70])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            for _ in range(5):
+                b.paged_attention(op)
+        work.append((graph, stream, b, c, q, out, op, keep))
+    for _ in range(5):
+        for graph, stream, *_ in work:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for graph, stream, b, c, q, out, op, keep in work:
+        want, size = attention64(c, q, [4, 70])
+        assert near(out, want, attention_tolerance("bf16", want, size, 9100))
+    del graph, work[:]
+    b.close()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dim,kv_heads", [(64, 2), (128, 2), (256, 1)])
+@pytest.mark.parametrize("new", [1, 2, 300])
+def test_scores_that_rise_from_tile_to_tile(be, dtype, dim, kv_heads, new):
+    """Each key's score is above the one before, by 0.2 for some rows and by 1.6 for others, down for the rest: the maximum of a tile of 128
+    is far above the last one's, up to e^200, so references are raised in every tile, and fall behind by less than that in others."""
+    group = 6
+    L = 1100
+    c = Cache([L, 40], kv_heads, dim, 16, dtype, seed=4)
+    step = torch.arange(L, device="cuda") / 256
+    c.key[0].zero_()
+    c.key[0][:, :, 0] = step[:, None].to(c.key[0].dtype)
+    for j, p in enumerate(c.pages[0]):
+        part = slice(j * 16, min(j * 16 + 16, L))
+        c.k[p, :part.stop - part.start] = c.key[0][part]
+    q = torch.zeros(new + 1, group * kv_heads, dim, device="cuda").to(DTYPE[dtype][0])
+    for h in range(group * kv_heads):
+        q[:, h, 0] = [50.0, 400.0, -400.0, 0.0, 10.0, 150.0][h % group]
+    out = torch.empty_like(q)
+    op, keep = attention_op(be, c, q, out, [new, 1], scale=1.0)
+    be.paged_attention(op)
+    want, size = attention64(c, q, [new, 1], scale=1.0)
+    # a score is one product below 2^11: formed exactly, and off by 2^-23 of it twice on its way to the exponent
+    tolerance = attention_tolerance(dtype, want, size, L) + 4 * 2.0 ** (11 - 23) * size
+    assert near(out, want, tolerance)
+
+
+def test_requests_with_a_common_prefix(be):
+    """The same pages in several rows, the same row for two requests: reading them is all that attention does."""
+    c = Cache([500, 500, 500], 2, 128, 16, "bf16")
+    for i in (1, 2):
+        c.table[c.rows_list[i], :20] = c.table[c.rows_list[0], :20]
+        c.key[i][:320], c.value[i][:320] = c.key[0][:320], c.value[0][:320]
+    c.rows[2] = c.rows[1]
+    c.key[2], c.value[2] = c.key[1], c.value[1]
+    check(be, c, 8, [1, 2, 1])
+    check(be, c, 8, [40, 1, 100])
+
+
 def test_offsets_beyond_32_bits(be):
     """A cache whose last pages lie behind 2^32 elements."""
     page, dim = 128, 256

@@ -263,6 +263,60 @@ def test_rope_far_positions_and_halves(be):
     assert (q_out == 0).all() and torch.equal(c.v[0, 5], x[0, 4:].half())
 
 
+@pytest.mark.parametrize("tokens,dim,rot,pairing,heads,kv_heads", [(297, 128, 128, 0, 1, 2), (591, 64, 16, 0, 9, 0), (593, 256, 256, 0, 2, 1), (2369, 256, 256, 1, 0, 1),
+                                                                   (4737, 64, 32, 0, 3, 1), (5000, 128, 36, 0, 2, 2)])
+@pytest.mark.parametrize("norms", ["none", "queries", "keys"])
+def test_rope_many_tokens(be, tokens, dim, rot, pairing, heads, kv_heads, norms):
+    """Blocks with one to eight tokens each, in one wave and more; one of the two norms; fewer query heads than KV heads, or none of either."""
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    x = torch.randn(tokens, heads + 2 * kv_heads, dim, generator=g, device="cuda").bfloat16()
+    positions = torch.arange(2 * tokens, device="cuda", dtype=torch.int32).reshape(2, tokens)
+    axis = torch.arange(rot // 2, device="cuda") % 2
+    c = Cache([tokens], max(kv_heads, 1), dim, 16, "bf16")
+    slots = torch.randperm(c.n_pages * 16, generator=g, device="cuda")[:tokens].int()
+    slots[tokens // 2] = -1
+    w = torch.randn(dim, generator=g, device="cuda") * 0.3 + 1
+    wq, wk = (w if norms == name else None for name in ("queries", "keys"))
+    q_out = torch.full((tokens, heads, dim), 9.0, device="cuda").bfloat16()
+    s = x.stride()
+    ptr = lambda t: None if t is None else t.data_ptr()
+    fields = dict(q=x.data_ptr(), q_out=q_out.data_ptr(), q_norm=ptr(wq)) if heads else {}
+    if kv_heads:
+        fields.update(k=x[:, heads:].data_ptr(), v=x[:, heads + kv_heads:].data_ptr(), k_norm=ptr(wk), slots=slots.data_ptr())
+    be.rope_append(ctox.RopeAppend(axis=axis.tolist(), tokens=tokens, heads=heads, kv_heads=kv_heads, dim=dim, rot_dim=rot, axes=2, pairing=pairing,
+                                   source_dtype=N.BF16, rope_base=1e4, positions=positions.data_ptr(), position_stride=tokens, q_token_stride=s[0],
+                                   q_head_stride=s[1], k_token_stride=s[0], k_head_stride=s[1], v_token_stride=s[0], v_head_stride=s[1],
+                                   norm_eps=1e-6, q_out_token_stride=q_out.stride(0), q_out_head_stride=q_out.stride(1), kv=c.op(), **fields))
+    torch.cuda.synchronize()
+    assert be.device_error() == 0
+    if heads:
+        want, size = rope64(x[:, :heads], wq, 0.0, 1e-6, positions, axis, 1e4, rot, pairing)
+        assert near(q_out, want, rope_tolerance("bf16", want, size))
+    if kv_heads:
+        want, size = rope64(x[:, heads:heads + kv_heads], wk, 0.0, 1e-6, positions, axis, 1e4, rot, pairing)
+        real = slots >= 0
+        place = slots[real].long()
+        assert near(c.k[place // 16, place % 16], want[real], rope_tolerance("bf16", want, size)[real])
+        assert torch.equal(c.v[place // 16, place % 16], x[real, heads + kv_heads:])
+
+
+def test_nothing_to_do(be):
+    """No tokens at all: no request brings any, and the arrays of tokens may be absent."""
+    m = Manager([5, 0], 16, 4, 8)
+    d = m.device()
+    op, o = slots_op(m, d, [0, 0], 0)
+    op.slots = op.positions = op.requests = None
+    be.page_slots(op)
+    c = Cache([5], 2, 128, 16, "bf16")
+    be.rope_append(ctox.RopeAppend(tokens=0, heads=2, kv_heads=2, dim=128, source_dtype=N.F32, q=c.k.data_ptr(), q_out=c.k.data_ptr(), kv=c.op()))
+    q = torch.zeros(1, 4, 128, device="cuda").bfloat16()
+    att, keep = attention_op(be, c, q, q, [0], max_new_tokens=0)
+    att.n_tokens, att.q, att.out = 0, None, None
+    be.paged_attention(att)
+    torch.cuda.synchronize()
+    assert be.device_error() == 0 and o["status"].tolist() == [0, 0] and o["offsets"].tolist() == [0, 0, 0] and d["lens"].tolist() == [5, 0]
+
+
 def test_rope_slots_out_of_range_are_left_out(be):
     c = Cache([20], 1, 64, 16, "bf16")
     x = torch.randn(3, 3, 64, device="cuda")
