@@ -29,7 +29,9 @@ struct Rows {
     static constexpr int MW = KM * SPLIT / NW;             // score tiles per warp
     static constexpr int KSTEPS = D / 16 / SPLIT;          // products of a score tile
     static constexpr int DW = D * NT / NW;                 // dimensions of a warp's output, for one group of eight rows
-    static constexpr int SP = KT + 8;                      // row pitch of the scores: keys and rows fall into different banks
+    // Row pitch of the scores: with eight more, keys and rows fall into different banks when they are read (with four, when they are written: 0 to 3 %
+    // slower). What is left for the line of 2048 requests beside the largest ring and scores wants four.
+    static constexpr int SP = KT + (D == 256 && NT == 2 ? 4 : 8);
     static constexpr uint32_t TILE = KT * D * 2;           // bytes of K or V
     static constexpr size_t SCORES = 2ull * SPLIT * BR * SP * 4;
     static size_t smem(uint32_t n) { return 1024 + (size_t)kStages * 2 * TILE + SCORES + (n + 1) * 8; }

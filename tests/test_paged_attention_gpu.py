@@ -144,6 +144,17 @@ def test_many_requests(be):
     check(be, Cache([lens[i] + m for i, m in enumerate(new)], 2, 128, 16, "f16"), 8, new)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_the_most_requests_in_every_kernel(be, dim):
+    """2048 requests leave the least shared memory: rows of 8, 16, more, and both kernels at once."""
+    lens = [1 + i % 29 for i in range(2048)]
+    c = Cache(lens, 1, dim, 16, "bf16")
+    check(be, c, 7, [1] * 2048)
+    check(be, c, 16, [1] * 2048)
+    check(be, c, 16, [1 + (i % 500 == 28) for i in range(2048)])
+    check(be, c, 16, [1 + (i % 500 == 28) for i in range(2048)], max_kv_tokens=3000)
+
+
 def test_bounds_that_are_larger_than_needed(be):
     """Captured programs name bounds for all of their replays."""
     check(be, Cache([40, 700], 2, 128, 16, "bf16"), 8, [1, 2], max_new_tokens=200, max_kv_tokens=100000)
