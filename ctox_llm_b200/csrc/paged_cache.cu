@@ -212,7 +212,7 @@ __device__ __forceinline__ void store4(T *p, const float *v) {
 // head with eight dimensions each, the norm's sum through shuffles. Both partners of a half-split pair are one lane's, so nothing is read twice.
 // Bound by latency and instructions as much as by memory: 4099 tokens of 16 + 4 + 4 heads of 128, 16 bits, take 16.7 us (3.1 TB/s), 19.3 with
 // one token's words under way per lane instead of two, 18.1 with CTAs in waves of unequal fill; 2475 tokens of 24 + 4 + 4 heads of 256 with norms
-// 25.6 us (3.2 TB/s), 30.1 in 2.1 waves. With few tokens several CTAs share a token's heads: 16 tokens take 4.0 us, mostly launch and dependent reads.
+// 25.9 us (3.1 TB/s), 30.1 in 2.1 waves. With few tokens several CTAs share a token's heads: 16 tokens take 4.0 us, mostly launch and dependent reads.
 constexpr uint32_t kRopeThreads = 256, kRopeTurns = 512, kRopeTokens = 8, kRopeResident = 4, kRopeTrips = 2;
 struct RopeRow {  // the heads of one kind of a token
     const void *x;
@@ -255,9 +255,12 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) k_rope_append(con
         const uint32_t t = i / pairs, p = i - t * pairs;
         // a far position times the fastest pair is thousands of turns
         const double x = (double)op.positions[op.axis[p] * op.position_stride + token0 + t] * a.turns[p];
+        // the angle in half turns as a sum of two numbers: sine and cosine of the first, and the slope times the second, which is below 2^-24
+        const double half_turns = 2.0 * (x - rint(x));
+        const float near = (float)half_turns, rest = (float)((half_turns - near) * 3.14159265358979323846);
         float sn, cs;
-        sincospif((float)(2.0 * (x - rint(x))), &sn, &cs);
-        turns[t * pairs + (paired ? ((p & 3) >> 1) * (pairs / 2) + (p >> 2) * 2 + (p & 1) : p)] = make_float2(cs, sn);
+        sincospif(near, &sn, &cs);
+        turns[t * pairs + (paired ? ((p & 3) >> 1) * (pairs / 2) + (p >> 2) * 2 + (p & 1) : p)] = make_float2(fmaf(-sn, rest, cs), fmaf(cs, rest, sn));
     }
     __syncthreads();
     const uint32_t q_heads = op.q ? op.heads : 0, heads = q_heads + (op.k ? 2 * op.kv_heads : 0);
@@ -309,9 +312,10 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) k_rope_append(con
 #pragma unroll
                     for (uint32_t o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                     if (normed) {
-                        inv = rsqrtf(sum * (1.f / D) + op.norm_eps);
+                        const float mean = sum * (1.f / D) + op.norm_eps, r = rsqrtf(mean);
+                        inv = fmaf(0.5f * r, fmaf(-mean * r, r, 1.f), r);  // one step of Newton's for the last bit
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] *= inv * w[j];
+                        for (int j = 0; j < 8; ++j) v[j] = v[j] * inv * w[j];
                     }
                 }
                 if (!out[n]) continue;
