@@ -8,6 +8,11 @@
 // padded to eight; one barrier per tile to exchange the scores; then every warp forms the weights that its share of the head's dimensions needs
 // (lane = row, redundantly: 32 exponentials per lane and tile) and adds V^T P for those dimensions. No output or maximum ever
 // crosses a warp.
+//
+// Measured: 48 sessions of up to 12000 tokens, 24 heads over 4 of 256, 800 MB of cache: 129 us with the merge (5 us), 6.2 TB/s; bound by
+// memory. One token of one session of 45: 9.6 us, bound by the start and four dependent reads. 17 to 32 rows would fit with one buffer of
+// scores, but wait for mma.sync: 24 rows on 32768 keys of 256 dimensions take 47.8 us, 42.1 on tcgen05; weights formed by every warp for all rows,
+// so that no value is read twice from shared memory, 66.
 #include "paged_attention.cuh"
 
 #include <cmath>
@@ -17,7 +22,7 @@ namespace paged {
 namespace {
 
 constexpr int kStages = 3;
-constexpr uint32_t kFewRows = 16;    // requests with more rows are paged_attention_tile.cu's
+constexpr uint32_t kFewRows = 16;    // requests with more rows are the other kernel's (above)
 
 template <int D, int NT>
 struct Rows {
