@@ -88,11 +88,11 @@ CTOX_HD Cuts cuts_of(uint64_t total, uint32_t ctas, uint32_t least) {
     c.least = least;
     c.pieces = total >= (uint64_t)least * ctas ? ctas : (uint32_t)total / least;
     if (!c.pieces && total) c.pieces = 1;
-    c.each = c.pieces ? total / c.pieces : 0;
+    c.each = !c.pieces ? 0 : total >> 32 ? total / c.pieces : (uint32_t)total / c.pieces;  // 64 bits take several times as long
     c.rest = (uint32_t)(total - c.each * c.pieces);
     return c;
 }
-CTOX_HD uint64_t raw_cut(const Cuts &c, uint32_t i) { return c.each * i + c.rest * i / c.pieces; }  // rest, i <= pieces: 32 bits
+CTOX_HD uint64_t raw_cut(const Cuts &c, uint32_t i) { return c.each * i + (i < c.rest ? i : c.rest); }  // the first `rest` are longer by one
 // A unit this short is not cut.
 CTOX_HD bool keeps_whole(uint32_t cost, uint32_t least) { return cost < 2 * least; }
 // CTAs that share a unit which starts in piece `first` and ends at `end`.
